@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define RB_NVFP4_ABI_VERSION 7
+#define RB_NVFP4_ABI_VERSION 8
 
 /* Input element types. */
 #define RB_DTYPE_BF16 0
@@ -40,6 +40,15 @@ extern "C" {
 /* Output element types of the GEMMs. */
 #define RB_OUT_BF16 0
 #define RB_OUT_F32 1
+
+/* Activations of the GEMM epilogue: z, max(z, 0), max(z, 0)^2, z / (1 + exp(-z)),
+ * z (1 + erf(z / sqrt 2)) / 2, z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2. */
+#define RB_ACT_NONE 0
+#define RB_ACT_RELU 1
+#define RB_ACT_RELU2 2
+#define RB_ACT_SILU 3
+#define RB_ACT_GELU 4
+#define RB_ACT_GELU_TANH 5
 
 /* Return codes. */
 #define RB_OK 0
@@ -350,6 +359,109 @@ int rb_nvfp4_gemm_grouped(const void* a_packed, const void* a_scale, int64_t a_r
                           const void* b_scale, int64_t b_rows, int64_t n, int64_t k_total, const int64_t* groups,
                           int num_groups, const float* alpha_a, const float* alpha_b, void* out, int out_dtype,
                           int64_t out_rows, int64_t ldo, void* stream);
+
+/*
+ * Counter-based dropout: y[i] = residual[i] + (kept(i) ? x[i] * 65536 / (65536 - t) : 0) for i < n,
+ * t = round(65536 p); the sum and the product in fp32, rounded once.  Element i is kept when the
+ * 16-bit half i % 2 of word (i % 8) / 2 of Philox4x32-10 with counter (i / 8, 0) and the seed as key is
+ * at least t.  The mask is a function of (seed, i) and is never stored: the backward pass is the same
+ * call on the upstream gradient (without residual), and rb_nvfp4_gemm_epilogue and
+ * rb_nvfp4_epilogue_backward draw the same mask for the same seed, i counting their rows x cols
+ * elements row-major.  A dropped element contributes 0 whatever x holds.  No counterpart in the
+ * reference (radiance uses nn.Dropout, src/radiance/model/ffn.py:10-39).
+ *   x, residual (NULL: none), y : n contiguous elements of `dtype`; y may be x or residual.
+ *   p    : 0 <= p <= 1; 0 keeps everything (seed unused), 1 drops everything.
+ *   seed : device int64, read on the device.
+ */
+int rb_nvfp4_dropout(const void* x, const void* residual, int dtype, int64_t n, double p, const int64_t* seed, void* y,
+                     void* stream);
+
+/*
+ * Backward of the epilogue y = residual + drop(act(z)) (rb_nvfp4_gemm_epilogue) in one pass over its
+ * inputs: grad_z = drop(grad_y) * act'(z) rounded to `dtype`; *gs_out = the global scale of the rounded
+ * grad_z as rb_nvfp4_global_scale computes it (quantize.py:205-213), for the quantizer of the backward
+ * GEMMs; and the bias gradient colsum_out[c] = sum over rows of the unrounded grad_z in fp32, in a
+ * fixed order (linear.py:146).  The gradient of the residual is grad_y itself.
+ *   grad_y, preact, grad_z : rows x cols of `dtype`, row strides ldg, ldz, ldo >= cols; preact NULL only
+ *               for RB_ACT_NONE.  Rows of 16-byte aligned multiples of 8 elements are read in vectors, others
+ *               element by element.  grad_z may be grad_y or preact (same strides).
+ *   p, seed   : as rb_nvfp4_dropout, with the seed of the forward call.
+ *   colsum_out: cols fp32, or NULL.
+ *   workspace : rb_nvfp4_epilogue_backward_workspace(rows, cols) bytes of scratch, 4-byte aligned; no
+ *               initial contents needed, nothing is kept in it.
+ */
+size_t rb_nvfp4_epilogue_backward_workspace(int64_t rows, int64_t cols);
+int rb_nvfp4_epilogue_backward(const void* grad_y, int64_t ldg, const void* preact, int64_t ldz, int dtype,
+                               int64_t rows, int64_t cols, int activation, double p, const int64_t* seed, void* grad_z,
+                               int64_t ldo, float* gs_out, float* colsum_out, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/*
+ * Mixture-of-experts routing (radiance's MoEFeedForward, src/radiance/model/ffn.py:156-436, does it with
+ * softmax, topk and index ops).  For every token: p = softmax(logits), its picks are the k experts of
+ * largest logit + expert_bias (compared in fp32; ties go to the lower expert, NaN counts as largest), and
+ * its weights are p of the picks, divided by their sum if `renormalize`.  An expert whose score is -inf
+ * is never picked: a token with fewer than k others gets picks of -1 with weight 0 for the rest, and a
+ * token without any, or with valid[t] == 0, is not routed at all (all picks -1; its logits are ignored).
+ *   counts[e]  : pairs (token, pick) of expert e;
+ *   offsets[e] : first row of expert e in the expert-sorted layout of rb_nvfp4_gemm_grouped, every group
+ *                padded to a multiple of 128 rows; offsets[experts] is its end;
+ *   rows[t, j] : the row of pair (t, j): offsets of its expert plus the number of that expert's pairs of
+ *                earlier tokens; -1 without a pick;
+ *   *loss      : E * sum_e (counts[e] / sum of counts) * (mean over the n routed tokens of p_e), 0 if n = 0;
+ *   *routed    : n.
+ *   logits : tokens x experts of `dtype`, row stride ld;  expert_bias : fp32[experts] or NULL;
+ *   valid  : one byte per token or NULL;  weights, picks, rows : tokens x k.
+ *   1 <= experts <= 256, 1 <= k <= min(experts, 32), tokens * k + 128 * experts < 2^31.
+ *   workspace : rb_nvfp4_route_workspace(tokens, experts, k) bytes of scratch, 4-byte aligned, no initial
+ *               contents needed.  Nothing is added in a varying order: results repeat bit for bit.
+ */
+size_t rb_nvfp4_route_workspace(int64_t tokens, int64_t experts, int k);
+int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
+                   const float* expert_bias, const void* valid, int renormalize, float* weights, int32_t* picks,
+                   int32_t* rows, int64_t* counts, int64_t* offsets, float* loss, int32_t* routed, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/*
+ * Gradient of rb_nvfp4_route's weights and loss with respect to the logits; the selection and the counts
+ * are constants.  With c_e = *grad_loss * E * (counts[e] / sum of counts) / n:
+ *   grad_logits = p (c - <p, c>) + the picks' part, w (g - <w, g>) at the picks if `renormalize`, else
+ *   w g at the picks minus p <w, g>;  rows of tokens that were not routed are 0.
+ *   grad_weights (tokens x k) and grad_loss (scalar) may each be NULL; grad_logits has the logits' dtype
+ *   and row stride ldo.
+ */
+int rb_nvfp4_route_backward(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
+                            int renormalize, const float* weights, const int32_t* picks, const int64_t* counts,
+                            const int32_t* routed, const float* grad_weights, const float* grad_loss,
+                            void* grad_logits, int64_t ldo, void* stream);
+
+/*
+ * Token rows to the expert-sorted layout: out[rows[t, j]] = x[t] for every pair with a row, and zero in
+ * every other row of out (the padding of each group, counts[e] .. offsets[e + 1], and everything from
+ * offsets[experts] to num_rows).  Rows at or past num_rows are skipped.  Every row of out is written.
+ *   x : tokens x d, row stride ldx;  out : num_rows x d, row stride ldo;  any d >= 1.
+ */
+int rb_nvfp4_token_dispatch(const void* x, int dtype, int64_t tokens, int64_t d, int64_t ldx, const int32_t* rows,
+                            int k, const int64_t* counts, const int64_t* offsets, int64_t experts, void* out,
+                            int64_t num_rows, int64_t ldo, void* stream);
+
+/*
+ * The weighted sum back: out[t] = residual[t] + sum_j weights[t, j] * y[rows[t, j]] over the pairs with a
+ * row, in fp32 and in the order of j, rounded once.  weights NULL: all 1, which is the backward of
+ * rb_nvfp4_token_dispatch.  residual may be NULL.
+ */
+int rb_nvfp4_token_combine(const void* y, int dtype, int64_t num_rows, int64_t d, int64_t ldy, const int32_t* rows,
+                           int k, const float* weights, const void* residual, int64_t ldr, void* out, int64_t tokens,
+                           int64_t ldo, void* stream);
+
+/*
+ * Backward of rb_nvfp4_token_combine: grad_rows[rows[t, j]] = weights[t, j] * grad_y[t], zero in every row
+ * without a pair, and grad_weights[t, j] = <grad_y[t], y[rows[t, j]]> (fp32, a fixed order; 0 without a row).
+ */
+int rb_nvfp4_token_combine_backward(const void* grad_y, int64_t ldg, const void* y, int64_t ldy, int dtype,
+                                    int64_t tokens, int64_t d, const int32_t* rows, int k, const float* weights,
+                                    const int64_t* counts, const int64_t* offsets, int64_t experts, void* grad_rows,
+                                    int64_t num_rows, int64_t ldo, float* grad_weights, void* stream);
 
 /*
  * Self-test of the quantizer's division: for i < n, compares the library's correctly rounded

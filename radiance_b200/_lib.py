@@ -17,6 +17,7 @@ from .build import LIB_PATH
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/radiance_nvfp4.h
 SIGNATURES: dict[str, tuple] = {
@@ -83,6 +84,39 @@ SIGNATURES: dict[str, tuple] = {
         _int, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64,
                _c_void_p, _c_void_p, _c_void_p],
     ),
+    "rb_nvfp4_dropout": (_int, [_c_void_p, _c_void_p, _int, _i64, _f64, _c_void_p, _c_void_p, _c_void_p]),
+    "rb_nvfp4_epilogue_backward_workspace": (ctypes.c_size_t, [_i64, _i64]),
+    "rb_nvfp4_epilogue_backward": (
+        _int,
+        [_c_void_p, _i64, _c_void_p, _i64, _int, _i64, _i64, _int, _f64, _c_void_p, _c_void_p, _i64, _c_void_p,
+         _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p],
+    ),
+    "rb_nvfp4_route_workspace": (ctypes.c_size_t, [_i64, _i64, _int]),
+    "rb_nvfp4_route": (
+        _int,
+        [_c_void_p, _int, _i64, _i64, _i64, _int, _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p],
+    ),
+    "rb_nvfp4_route_backward": (
+        _int,
+        [_c_void_p, _int, _i64, _i64, _i64, _int, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p, _i64, _c_void_p],
+    ),
+    "rb_nvfp4_token_dispatch": (
+        _int,
+        [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _int, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64,
+         _c_void_p],
+    ),
+    "rb_nvfp4_token_combine": (
+        _int,
+        [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _int, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64,
+         _c_void_p],
+    ),
+    "rb_nvfp4_token_combine_backward": (
+        _int,
+        [_c_void_p, _i64, _c_void_p, _i64, _int, _i64, _i64, _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p, _i64,
+         _c_void_p, _i64, _i64, _c_void_p, _c_void_p],
+    ),
     "rb_nvfp4_selftest_wait_timeout": (_int, [_int, ctypes.c_longlong, _c_void_p, _c_void_p]),
     "rb_peer_alloc": (_int, [ctypes.c_size_t, ctypes.POINTER(_c_void_p)]),
     "rb_peer_free": (_int, [_c_void_p]),
@@ -93,12 +127,13 @@ SIGNATURES: dict[str, tuple] = {
 
 RB_PEER_HANDLE_BYTES = 64
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 RB_DTYPE_BF16 = 0
 RB_DTYPE_F32 = 1
 RB_OUT_BF16 = 0
 RB_OUT_F32 = 1
+RB_ACTIVATIONS = {None: 0, "relu": 1, "relu2": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}
 
 _ERRORS = {1: ValueError, 2: ValueError, 3: RuntimeError, 4: RuntimeError}
 

@@ -1,0 +1,202 @@
+"""What follows a linear's product in a feed-forward sublayer: activation, dropout and residual.
+
+radiance's ``FeedForward`` ends in ``nn.Dropout`` and its block adds the residual
+(src/radiance/model/ffn.py:10-39, block.py:45-71), each a full pass over the output.  Here they run
+where the product is (``epilogue_mm``), their backward is one pass that also yields what the
+linear's backward needs of the gradient (``epilogue_backward``), and ``dropout`` stands alone for
+outputs of other producers.
+
+The dropout mask is a function of a 64-bit seed and the element's row-major index (Philox4x32-10),
+drawn where it is needed and never stored; the three operators draw the same mask for the same seed.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from . import _trace
+from .quantize import _require_cuda, _stream_ptr
+
+_DTYPES = {torch.bfloat16: _lib.RB_DTYPE_BF16, torch.float32: _lib.RB_DTYPE_F32}
+
+
+def _dtype_of(x: torch.Tensor, what: str) -> int:
+    code = _DTYPES.get(x.dtype)
+    if code is None:
+        raise ValueError(f"{what}: unsupported dtype {x.dtype} (bf16 or fp32)")
+    return code
+
+
+def _call(what: str, device: torch.device, fn, *args) -> None:
+    """One C call (its stream argument appended) with ``device`` current, and its error raised."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, _stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _stream_ptr(device))
+    if rc:
+        _lib.check(rc, what)
+
+
+def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """A 2-D tensor whose rows are contiguous and do not overlap, and its row stride in elements."""
+    r, c = x.shape
+    if (c > 1 and x.stride(1) != 1) or (r > 1 and x.stride(0) < c):
+        x = x.contiguous()
+    return x, (x.stride(0) if r > 1 else c)
+
+
+def _like(name: str, t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device, what: str) -> None:
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{what}: {name} must be {dtype} of shape {tuple(shape)} on {device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+
+
+def _probability(p: float, what: str) -> float:
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{what}: the dropout probability must be in [0, 1], got {p}")
+    return p
+
+
+def dropout_seed(device: torch.device | str = "cuda") -> torch.Tensor:
+    """A fresh dropout seed (0-d int64) from torch's CUDA generator: it follows ``torch.manual_seed``, the
+    generator state that activation checkpointing restores, and replays of a captured graph."""
+    return torch.empty((), dtype=torch.int64, device=device).random_()
+
+
+def _seed_tensor(seed: torch.Tensor | int | None, device: torch.device, what: str) -> torch.Tensor:
+    if seed is None:
+        return dropout_seed(device)
+    if not isinstance(seed, torch.Tensor):
+        return torch.full((), int(seed), dtype=torch.int64, device=device)
+    if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
+        raise ValueError(f"{what}: seed must be an int or one int64 on {device}, got {seed.dtype} "
+                         f"{tuple(seed.shape)} on {seed.device}")
+    return seed
+
+
+# ------------------------------------------------------------------------------------------------
+# Dropout
+# ------------------------------------------------------------------------------------------------
+
+
+def _dropout(x: torch.Tensor, residual: torch.Tensor | None, p: float, seed: torch.Tensor | None) -> torch.Tensor:
+    what = "nvfp4.dropout"
+    code = _dtype_of(x, what)
+    x = x.contiguous()
+    if residual is not None:
+        residual = residual.contiguous()
+    y = torch.empty_like(x)
+    n = x.numel()
+    tok = _trace.begin("dropout", n * x.element_size() * (2 + (residual is not None)))
+    _call(what, x.device, _lib.load().rb_nvfp4_dropout, x.data_ptr(),
+          None if residual is None else residual.data_ptr(), code, n, p, None if seed is None else seed.data_ptr(),
+          y.data_ptr())
+    _trace.end(tok)
+    return y
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed):
+        ctx.p = p
+        ctx.save_for_backward(seed)
+        return _dropout(x, residual, p, seed)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        (seed,) = ctx.saved_tensors
+        gx = None
+        if ctx.needs_input_grad[0]:
+            gx = grad if seed is None else _dropout(grad, None, ctx.p, seed)
+        return gx, (grad if ctx.needs_input_grad[1] else None), None, None
+
+
+def dropout(x: torch.Tensor, p: float = 0.5, *, seed: torch.Tensor | int | None = None,
+            residual: torch.Tensor | None = None, training: bool = True) -> torch.Tensor:
+    """``residual + drop(x)`` in one pass (``residual`` optional), differentiable in both.
+
+    An element is dropped with probability ``t / 65536``, ``t = round(65536 p)``; a kept one is
+    multiplied by ``65536 / (65536 - t)``, a dropped one contributes 0 whatever it holds.  bf16 or
+    fp32, any shape; product and sum in fp32, rounded once.  ``seed``: an int, a 0-d int64 CUDA
+    tensor (read on the device, so a captured graph can change it; it must keep its value until the
+    backward pass, which draws the mask again), or None for a fresh ``dropout_seed``.  Equal seeds
+    give equal masks for equal element counts.
+    """
+    what = "nvfp4.dropout"
+    _require_cuda(x, what)
+    _dtype_of(x, what)
+    p = _probability(p, what) if training else 0.0
+    if residual is not None:
+        _like("residual", residual, x.shape, x.dtype, x.device, what)
+    if p == 0.0 and residual is None:
+        return x
+    seed = _seed_tensor(seed, x.device, what) if p > 0.0 else None
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return _DropoutFn.apply(x, residual, p, seed)
+    return _dropout(x, residual, p, seed)
+
+
+# ------------------------------------------------------------------------------------------------
+# The backward of the GEMM epilogue
+# ------------------------------------------------------------------------------------------------
+
+
+def _activation_code(activation: str | None, what: str) -> int:
+    code = _lib.RB_ACTIVATIONS.get(activation)
+    if code is None:
+        names = ", ".join(repr(a) for a in _lib.RB_ACTIVATIONS)
+        raise ValueError(f"{what}: activation must be one of {names}, got {activation!r}")
+    return code
+
+
+def epilogue_backward(grad_y: torch.Tensor, preact: torch.Tensor | None = None, *, activation: str | None = None,
+                      dropout_p: float = 0.0, seed: torch.Tensor | int | None = None, bias_grad: bool = False,
+                      out: torch.Tensor | None = None
+                      ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """The gradient of ``epilogue_mm``'s pre-activations: ``grad_z = drop(grad_y) * act'(preact)``.
+
+    One pass over ``grad_y`` and ``preact`` (2-D, the same dtype) that also takes the global scale of
+    ``grad_z``, which the quantizer of the backward GEMMs needs, and with ``bias_grad`` its fp32 column
+    sums.  ``seed`` is the forward call's.  Returns ``(grad_z, global_scale_of(grad_z), sums or None)``.
+    The gradient of the residual is ``grad_y`` itself.
+    """
+    what = "nvfp4.epilogue_backward"
+    _require_cuda(grad_y, what)
+    code, act = _dtype_of(grad_y, what), _activation_code(activation, what)
+    p = _probability(dropout_p, what)
+    if grad_y.dim() != 2 or grad_y.numel() == 0:
+        raise ValueError(f"{what}: a non-empty 2-D gradient expected, got shape {tuple(grad_y.shape)}")
+    dev, (rows, cols) = grad_y.device, grad_y.shape
+    grad_y, ldg = _rows(grad_y)
+    z, ldz = None, cols
+    if act:
+        if preact is None:
+            raise ValueError(f"{what}: activation {activation!r} needs the pre-activations")
+        _like("preact", preact, (rows, cols), grad_y.dtype, dev, what)
+        z, ldz = _rows(preact)
+    if p > 0.0:
+        if seed is None:
+            raise ValueError(f"{what}: dropout needs the forward call's seed")
+        seed = _seed_tensor(seed, dev, what)
+    if out is None:
+        out = torch.empty(rows, cols, dtype=grad_y.dtype, device=dev)
+    else:
+        _like("out", out, (rows, cols), grad_y.dtype, dev, what)
+        if _rows(out)[0] is not out:
+            raise ValueError(f"{what}: out must have contiguous rows")
+    gs = torch.empty((), dtype=torch.float32, device=dev)
+    sums = torch.empty(cols, dtype=torch.float32, device=dev) if bias_grad else None
+    lib = _lib.load()
+    need = int(lib.rb_nvfp4_epilogue_backward_workspace(rows, cols))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    tok = _trace.begin("epilogue", rows * cols * grad_y.element_size() * (2 + (z is not None)))
+    _call(what, dev, lib.rb_nvfp4_epilogue_backward, grad_y.data_ptr(), ldg, None if z is None else z.data_ptr(), ldz,
+          code, rows, cols, act, p, seed.data_ptr() if p > 0.0 else None, out.data_ptr(), _rows(out)[1], gs.data_ptr(),
+          None if sums is None else sums.data_ptr(), ws.data_ptr(), need)
+    _trace.end(tok)
+    return out, gs, sums
