@@ -361,6 +361,24 @@ int rb_nvfp4_gemm_grouped(const void* a_packed, const void* a_scale, int64_t a_r
                           int64_t out_rows, int64_t ldo, void* stream);
 
 /*
+ * rb_nvfp4_gemm with the rest of a sublayer in its epilogue: z = alpha_a alpha_b A B^T + bias,
+ * out = residual + drop(act(z)), everything in fp32 from the accumulator on and rounded once to out_dtype
+ * (radiance runs nn.Dropout and the block's residual add as passes of their own, src/radiance/model/ffn.py:10-39,
+ * block.py:45-71).
+ *   activation : RB_ACT_*, evaluated on the unrounded z.
+ *   p, seed    : dropout as rb_nvfp4_dropout, element (i, j) having index i * n + j.
+ *   residual   : m x n of out_dtype, row stride ldr, or NULL.  out may be the residual itself (same pointer
+ *                and stride); any other overlap of out, preact and residual is not allowed.
+ *   preact     : NULL, or where z (rounded to out_dtype) is stored for rb_nvfp4_epilogue_backward, row stride ldz.
+ *   All 16-byte aligned with 16-byte row strides; shapes as rb_nvfp4_gemm.
+ */
+int rb_nvfp4_gemm_epilogue(const void* a_packed, const void* a_scale, const void* b_packed, const void* b_scale,
+                           int64_t m, int64_t n, int64_t k, const float* alpha_a, const float* alpha_b,
+                           const void* bias, int bias_dtype, int activation, double p, const int64_t* seed,
+                           const void* residual, int64_t ldr, void* preact, int64_t ldz, void* out, int out_dtype,
+                           int64_t ldo, void* stream);
+
+/*
  * Counter-based dropout: y[i] = residual[i] + (kept(i) ? x[i] * 65536 / (65536 - t) : 0) for i < n,
  * t = round(65536 p); the sum and the product in fp32, rounded once.  Element i is kept when the
  * 16-bit half i % 2 of word (i % 8) / 2 of Philox4x32-10 with counter (i / 8, 0) and the seed as key is

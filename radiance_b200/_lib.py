@@ -84,6 +84,11 @@ SIGNATURES: dict[str, tuple] = {
         _int, [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64,
                _c_void_p, _c_void_p, _c_void_p],
     ),
+    "rb_nvfp4_gemm_epilogue": (
+        _int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _int, _int,
+         _f64, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _int, _i64, _c_void_p],
+    ),
     "rb_nvfp4_dropout": (_int, [_c_void_p, _c_void_p, _int, _i64, _f64, _c_void_p, _c_void_p, _c_void_p]),
     "rb_nvfp4_epilogue_backward_workspace": (ctypes.c_size_t, [_i64, _i64]),
     "rb_nvfp4_epilogue_backward": (

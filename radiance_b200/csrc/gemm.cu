@@ -24,6 +24,7 @@
 // columns first and releases them, so the next tile's MMAs start while the rest drains.
 // No TMA multicast is used (the same kernel serves multi-GPU jobs).
 #include "common.cuh"
+#include "epilogue.cuh"
 #include "../../include/radiance_nvfp4.h"
 
 namespace rb {
@@ -91,6 +92,11 @@ struct GemmArgs {
   int64_t ldh;
   uint32_t* h_ws;  // {max |h| as bf16 bits, finished epilogue warps}: zero on entry, left zero
   float* h_gs;
+  // Fused epilogue (the two-SM kernel's kFused instantiation): y = residual + drop(act(z)) is stored to
+  // the output and, with has_preact, z to the tensor of the map in h's place.
+  int act;
+  int has_residual, has_preact;
+  DropoutArgs drop;
 };
 
 constexpr int kMaxPeers = 7;
@@ -739,43 +745,53 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 // =============================================================================================
 constexpr int kSfStep = 2048;  // one K step's scale atoms for 128 rows (4 x 512 B)
 
+// What the epilogue does besides alpha, bias and the cast.
+constexpr int kPlain = 0;
+constexpr int kSwigluMode = 1;  // also h = silu(g) * u and its maximum (rb_nvfp4_gemm_swiglu)
+constexpr int kFused = 2;       // activation, dropout, residual (rb_nvfp4_gemm_epilogue)
+
 // Per instantiation: the plain GEMM keeps five operand stages and four epilogue warps.  The SwiGLU
 // GEMM's epilogue also computes and stores h, so it runs two epilogue warps on each TMEM lane
 // quarter -- eight in all, two per scheduler, each taking every other 64-column chunk -- and pays
 // for their staging boxes, the h boxes and the silu table with one stage less.  Measured at 16384 x
 // 11264 x 2048: four stages with one (output, h) box pair per warp 211 us; three stages 231 us with
-// one pair or two.
-template <bool kSwiglu>
+// one pair or two.  The fused epilogue computes as much per element (an activation, a generator call
+// for eight elements) and takes the same split, with two boxes per warp.
+template <int kMode>
 struct Gemm2Cfg {
-  static constexpr int kStages = kSwiglu ? 4 : 5;
-  static constexpr int kEpiWarps = kSwiglu ? 8 : 4;
+  static constexpr int kStages = kMode != kPlain ? 4 : 5;
+  static constexpr int kEpiWarps = kMode != kPlain ? 8 : 4;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;  // producer, MMA issuer, epilogue
   static constexpr int kSwBoxes = 1;                    // SwiGLU mode: staged (output, h) box pairs per warp
+  static constexpr int kOutBoxes = kMode == kSwigluMode ? kEpiWarps * kSwBoxes : 2 * kEpiWarps;
+  static constexpr int kHBoxes = kMode == kSwigluMode ? kEpiWarps * kSwBoxes : 1;
 };
 
-template <bool kSwiglu>
+template <int kMode>
 struct Gemm2Smem {
-  static constexpr int S = Gemm2Cfg<kSwiglu>::kStages;
+  static constexpr int S = Gemm2Cfg<kMode>::kStages;
   uint8_t a[S][kBM * kStepBytes];  // this CTA's 128 A rows (16 KB)
   uint8_t b[S][kBM * kStepBytes];  // this CTA's 128 of the tile's 256 B rows (16 KB)
   uint8_t sfa[S][kSfStep];         // scale atoms of this CTA's A rows
   uint8_t sfb[S][2 * kSfStep];     // scale atoms of all 256 B rows: [half][k block]
   // Staged output boxes: two per epilogue warp, or kSwBoxes per warp in SwiGLU mode, with as many h
   // boxes.
-  uint8_t out[kSwiglu ? Gemm2Cfg<kSwiglu>::kEpiWarps * Gemm2Cfg<kSwiglu>::kSwBoxes : 8][4096];
-  uint8_t hbox[kSwiglu ? Gemm2Cfg<kSwiglu>::kEpiWarps * Gemm2Cfg<kSwiglu>::kSwBoxes : 1][kSwiglu ? 2048 : 16];
-  uint16_t silu_tab[kSwiglu ? 2 * kSiluTab : 8];        // SwiGLU mode: the silu table
+  uint8_t out[Gemm2Cfg<kMode>::kOutBoxes][4096];
+  uint8_t hbox[Gemm2Cfg<kMode>::kHBoxes][kMode == kSwigluMode ? 2048 : 16];
+  uint16_t silu_tab[kMode == kSwigluMode ? 2 * kSiluTab : 8];  // SwiGLU mode: the silu table
   int tile_prefix[kMaxGroups + 1];  // grouped mode: tiles of groups 0..g-1
   uint64_t full[S];                 // leader: both CTAs' loads of a stage
   uint64_t empty[S];                // each CTA: the leader's MMAs finished with a stage
   uint64_t acc_full;                // each CTA: the accumulator of a tile is complete
   uint64_t acc_empty;               // leader: the pair's epilogue warps are done with the shared columns
   uint64_t drain;
+  uint64_t res_full[kMode == kFused ? Gemm2Cfg<kMode>::kOutBoxes : 1];  // fused: a residual box has landed
   uint32_t tmem_base;
 };
 
 // Dynamic shared memory is the struct plus 1 KB for the 1024-byte alignment; 227 KB per CTA at most.
-static_assert(sizeof(Gemm2Smem<false>) + 1024 <= 232448 && sizeof(Gemm2Smem<true>) + 1024 <= 232448,
+static_assert(sizeof(Gemm2Smem<kPlain>) + 1024 <= 232448 && sizeof(Gemm2Smem<kSwigluMode>) + 1024 <= 232448 &&
+                  sizeof(Gemm2Smem<kFused>) + 1024 <= 232448,
               "two-SM GEMM shared memory exceeds 227 KB");
 
 constexpr uint32_t kStageBytes2 = 2 * kBM * kStepBytes + 3 * kSfStep;  // per CTA
@@ -906,16 +922,214 @@ __device__ __forceinline__ Tile2 tile2_at(int t, const GemmArgs& g, const int* p
   return T;
 }
 
-template <bool kSwiglu>
-__global__ void __launch_bounds__(Gemm2Cfg<kSwiglu>::kThreads, 1)
+// ---------------------------------------------------------------------------------------------
+// Fused epilogue: y = residual + drop(act(z)), z = alpha acc + bias
+// ---------------------------------------------------------------------------------------------
+
+// 16-byte chunk c of this lane's row of a staged box (128-byte swizzle).
+__device__ __forceinline__ uint32_t box_chunk(uint32_t row_addr, int c, uint32_t sw) {
+  return row_addr + (((uint32_t)c ^ sw) << 4);
+}
+
+// Eight values as one (bf16) or two (fp32) chunks, numbered by the eight-column group j of the box.
+__device__ __forceinline__ void box_store8(const float (&v)[8], uint32_t row_addr, int j, uint32_t sw, bool f32) {
+  if (f32) {
+    st_shared_v4(box_chunk(row_addr, 2 * j, sw), __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                 __float_as_uint(v[3]));
+    st_shared_v4(box_chunk(row_addr, 2 * j + 1, sw), __float_as_uint(v[4]), __float_as_uint(v[5]),
+                 __float_as_uint(v[6]), __float_as_uint(v[7]));
+  } else {
+    st_shared_v4(box_chunk(row_addr, j, sw), pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                 pack_bf16x2(v[6], v[7]));
+  }
+}
+__device__ __forceinline__ void box_add8(float (&v)[8], uint32_t row_addr, int j, uint32_t sw, bool f32) {
+  if (f32) {
+    const uint4 a = ld_shared_v4(box_chunk(row_addr, 2 * j, sw)), b = ld_shared_v4(box_chunk(row_addr, 2 * j + 1, sw));
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += __uint_as_float(w[i]);
+  } else {
+    const uint4 a = ld_shared_v4(box_chunk(row_addr, j, sw));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] += __uint_as_float(w[i] << 16);
+      v[2 * i + 1] += __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+}
+
+template <int kAct>
+__device__ __forceinline__ void act8(float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = act_value<kAct>(v[i]);
+}
+
+// 32 accumulator columns of this lane's row (r), columns col0 .. col0 + 31 of the output, at the box's
+// eight-column groups j0 .. j0 + 3.  The residual lies in the box where the result goes, so each lane
+// replaces its own chunks and needs no one else's.
+__device__ __forceinline__ void fused_columns(const uint32_t* r, float alpha, const GemmArgs& g, int64_t row, int col0,
+                                              PhiloxKey key, uint32_t row_addr, uint32_t zrow_addr, int j0,
+                                              uint32_t sw) {
+  const bool f32 = g.out_f32 != 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int col = col0 + 8 * j;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__uint_as_float(r[8 * j + i]), alpha);
+    if (g.bias != nullptr) {
+      float b[8];
+      if (g.bias_f32) Io<float>::load8(b, reinterpret_cast<const float*>(g.bias) + col);
+      else Io<__nv_bfloat16>::load8(b, reinterpret_cast<const __nv_bfloat16*>(g.bias) + col);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __fadd_rn(v[i], b[i]);
+    }
+    if (g.has_preact) box_store8(v, zrow_addr, j0 + j, sw, f32);
+    switch (g.act) {
+      case RB_ACT_RELU: act8<RB_ACT_RELU>(v); break;
+      case RB_ACT_RELU2: act8<RB_ACT_RELU2>(v); break;
+      case RB_ACT_SILU: act8<RB_ACT_SILU>(v); break;
+      case RB_ACT_GELU: act8<RB_ACT_GELU>(v); break;
+      case RB_ACT_GELU_TANH: act8<RB_ACT_GELU_TANH>(v); break;
+      default: break;
+    }
+    if (g.drop.seed != nullptr) dropout8(v, (uint64_t)(row * g.N + col) >> 3, key, g.drop.threshold, g.drop.scale);
+    if (g.has_residual) box_add8(v, row_addr, j0 + j, sw, f32);
+    box_store8(v, row_addr, j0 + j, sw, f32);
+  }
+}
+
+// One epilogue warp of the two-SM kernel in fused mode.  Its work is a sequence of pieces, one box (32
+// rows x 128 bytes: 64 bf16 or 32 fp32 columns) each.  The residual of a piece is loaded by TMA into the
+// box that the piece is staged in, replaced there element by element and stored by TMA.  The warp's two
+// boxes alternate, and while one piece is computed the next one's residual (the next tile's, after the
+// last) is on its way; with the pre-activations kept, the second box holds them and the residual is
+// loaded when its piece begins.
+template <class Smem>
+__device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, const CUtensorMap& tmO,
+                                               const CUtensorMap& tmZ, const CUtensorMap& tmR, int cid, int ncl,
+                                               int n_my, uint32_t rank, int warp, int lane) {
+  const int q = warp & 3, ew = warp - 2, half = ew / 4;
+  const uint32_t boxes = smem_u32(&sm.out[2 * ew][0]);
+  uint64_t* bars = &sm.res_full[2 * ew];
+  const bool f32 = g.out_f32 != 0, residual = g.has_residual != 0, preact = g.has_preact != 0;
+  const bool ahead = residual && !preact;  // residuals are loaded one piece ahead
+  const int parts = f32 ? 2 : 1;           // pieces of a 64-column chunk
+  const PhiloxKey key = g.drop.seed != nullptr ? philox_key(g.drop.seed) : PhiloxKey{0, 0};
+  const uint32_t sw = (uint32_t)(lane & 7), lane_row = (uint32_t)lane * 128u;
+  const auto row_of = [&](const Tile2& T) { return T.orow + (int64_t)rank * kBM + 32 * q; };
+  // The 64-column chunk that tile i's shared columns [192, 256) hold, or -1 (see the plain epilogue).
+  const auto shared_chunk = [&](int i, int width) { return (i & 1) ? 0 : (width == kBN ? width / kEpiChunk - 1 : -1); };
+  // This warp's chunk at `step` of tile i: ascending, except that buffer 0's shared last chunk goes first.
+  const auto chunk_at = [&](int i, int width, int step) {
+    const int sc = shared_chunk(i, width);
+    const bool first = sc >= 0 && (sc & 1) == half && !(i & 1);
+    return first ? (step == 0 ? sc : half + (step - 1) * 2) : half + step * 2;
+  };
+  const auto load_residual = [&](int slot, int64_t row, int col) {
+    mbar_arrive_expect_tx(&bars[slot], kOutBox);
+    tma_load_2d(reinterpret_cast<void*>(&sm.out[2 * ew + slot][0]), &tmR, &bars[slot], col, (int)row);
+  };
+  Tile2 T = tile2_at(cid, g, sm.tile_prefix);
+  uint32_t phases = 0;  // bit s: the parity that box s's next residual completes
+  int slot = 0;
+  if (ahead && n_my > 0 && lane == 0 && row_of(T) < T.row_end)
+    load_residual(0, row_of(T), T.ncol0 + chunk_at(0, T.width, 0) * kEpiChunk);
+  for (int i = 0; i < n_my; ++i) {
+    const Tile2 Tn = i + 1 < n_my ? tile2_at(cid + (i + 1) * ncl, g, sm.tile_prefix) : T;
+    float alpha = 1.0f;
+    if (g.alpha_a != nullptr) alpha = __ldg(g.alpha_a);
+    if (g.alpha_b != nullptr) alpha = __fmul_rn(alpha, __ldg(g.alpha_b));
+    if (!__all_sync(0xFFFFFFFFu, mbar_wait_sleep(&sm.acc_full, (uint32_t)(i & 1), 64))) {
+      if (lane == 0) record_status(&g_gemm_status, kStatusTimeoutMma);
+      return;
+    }
+    tc_fence_after();
+    const int base_col = (i & 1) ? kAcc1Col : 0;
+    const int sc = shared_chunk(i, T.width);
+    const bool mine_sc = sc >= 0 && (sc & 1) == half;
+    const auto release = [&]() {
+      if (rank == 0) mbar_arrive(&sm.acc_empty);
+      else mbar_arrive_leader(&sm.acc_empty);
+    };
+    if (!mine_sc && lane == 0) release();
+    const int64_t row0 = row_of(T);
+    const bool store = row0 < T.row_end;
+    const int nmine = T.width / (2 * kEpiChunk);
+    for (int step = 0; step < nmine; ++step) {
+      const int c = chunk_at(i, T.width, step);
+      uint32_t r[kEpiChunk];
+      const uint32_t taddr = ((uint32_t)(32 * q) << 16) + (uint32_t)(base_col + c * kEpiChunk);
+      RB_TMEM_LD_X32(taddr, r);
+      RB_TMEM_LD_X32(taddr + 32, (r + 32));
+      tmem_ld_wait();
+      if (step == 0 && mine_sc) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) release();
+      }
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        if (part >= parts) break;
+        const int col0 = T.ncol0 + c * kEpiChunk + 32 * part;
+        if (lane == 0) {
+          // The box to write into (or to load the next residual into) is read by no store any more.
+          if (residual || preact) bulk_wait_read<0>();
+          else bulk_wait_read<1>();
+          if (ahead) {
+            if (part + 1 < parts) {
+              if (store) load_residual(slot ^ 1, row0, col0 + 32);
+            } else if (step + 1 < nmine) {
+              if (store) load_residual(slot ^ 1, row0, T.ncol0 + chunk_at(i, T.width, step + 1) * kEpiChunk);
+            } else if (i + 1 < n_my && row_of(Tn) < Tn.row_end) {
+              load_residual(slot ^ 1, row_of(Tn), Tn.ncol0 + chunk_at(i + 1, Tn.width, 0) * kEpiChunk);
+            }
+          } else if (residual && store) {
+            load_residual(0, row0, col0);
+          }
+        }
+        __syncwarp();
+        if (residual && store) {
+          if (!mbar_wait_warp(&bars[slot], (phases >> slot) & 1u)) {
+            if (lane == 0) record_status(&g_gemm_status, kStatusTimeoutTma);
+            return;
+          }
+          phases ^= 1u << slot;
+        }
+        const uint32_t row_addr = boxes + (uint32_t)slot * kOutBox + lane_row, zrow_addr = boxes + kOutBox + lane_row;
+        if (f32) {
+          fused_columns(r + 32 * part, alpha, g, row0 + lane, col0, key, row_addr, zrow_addr, 0, sw);
+        } else {
+          fused_columns(r, alpha, g, row0 + lane, col0, key, row_addr, zrow_addr, 0, sw);
+          fused_columns(r + 32, alpha, g, row0 + lane, col0 + 32, key, row_addr, zrow_addr, 4, sw);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && store) {
+          tma_store_2d(&tmO, boxes + (uint32_t)slot * kOutBox, col0, (int)row0);
+          if (preact) tma_store_2d(&tmZ, boxes + kOutBox, col0, (int)row0);
+          bulk_commit_group();
+        }
+        if (!preact) slot ^= 1;
+      }
+    }
+    T = Tn;
+  }
+}
+
+template <int kMode>
+__global__ void __launch_bounds__(Gemm2Cfg<kMode>::kThreads, 1)
     nvfp4_gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
                        const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmH,
-                       const GemmArgs g) {
+                       const __grid_constant__ CUtensorMap tmR, const GemmArgs g) {
   extern __shared__ uint8_t smem_raw[];
-  using Smem = Gemm2Smem<kSwiglu>;
-  constexpr int kS = Gemm2Cfg<kSwiglu>::kStages;
-  constexpr int kEW = Gemm2Cfg<kSwiglu>::kEpiWarps;
+  constexpr bool kSwiglu = kMode == kSwigluMode;
+  using Smem = Gemm2Smem<kMode>;
+  constexpr int kS = Gemm2Cfg<kMode>::kStages;
+  constexpr int kEW = Gemm2Cfg<kMode>::kEpiWarps;
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -954,6 +1168,8 @@ __global__ void __launch_bounds__(Gemm2Cfg<kSwiglu>::kThreads, 1)
     mbar_init(&sm.acc_full, 1);
     mbar_init(&sm.acc_empty, 2 * kEW);
     mbar_init(&sm.drain, 1);
+    if constexpr (kMode == kFused)
+      for (int b = 0; b < Gemm2Cfg<kMode>::kOutBoxes; ++b) mbar_init(&sm.res_full[b], 1);
     fence_mbar_init();
     prefetch_tensormap(&tmA);
     prefetch_tensormap(&tmB);
@@ -961,6 +1177,10 @@ __global__ void __launch_bounds__(Gemm2Cfg<kSwiglu>::kThreads, 1)
     prefetch_tensormap(&tmSB);
     prefetch_tensormap(&tmO);
     if constexpr (kSwiglu) prefetch_tensormap(&tmH);
+    if constexpr (kMode == kFused) {
+      if (g.has_preact) prefetch_tensormap(&tmH);
+      if (g.has_residual) prefetch_tensormap(&tmR);
+    }
   }
   if (warp == 1) {
     tmem_alloc2(&sm.tmem_base, 512);
@@ -1088,9 +1308,12 @@ __global__ void __launch_bounds__(Gemm2Cfg<kSwiglu>::kThreads, 1)
     const int q = warp & 3;  // TMEM lanes 32q .. 32q+31
     constexpr int kStride = kEW / 4;
     const int half = (warp - 2) / 4;
+    if constexpr (kMode == kFused) {
+      fused_epilogue(sm, g, tmO, tmH, tmR, cid, ncl, n_my, rank, warp, lane);
+    } else {
     // Staging: two boxes per warp (pieces alternate between them), or in SwiGLU mode kSwBoxes
     // (output, h) box pairs per warp.
-    constexpr int kBoxes = kSwiglu ? Gemm2Cfg<kSwiglu>::kSwBoxes : 2;
+    constexpr int kBoxes = kSwiglu ? Gemm2Cfg<kMode>::kSwBoxes : 2;
     const uint32_t slots = smem_u32(&sm.out[(kSwiglu ? warp - 2 : q) * kBoxes][0]);
     int slot = 0;
     uint32_t hmax = 0;  // SwiGLU mode: this lane's max |h| (bf16 bits)
@@ -1149,6 +1372,7 @@ __global__ void __launch_bounds__(Gemm2Cfg<kSwiglu>::kThreads, 1)
       }
     }
     if constexpr (kSwiglu) swiglu_finish(g, hmax, gridDim.x * (uint32_t)kEW, lane);
+    }
     if (lane == 0) bulk_wait_all();
     if (g.npeers > 0) __threadfence_system();
     __syncwarp();
@@ -1174,10 +1398,10 @@ namespace {
 // Launches the two-SM kernel on min(clusters_wanted, resident clusters) CTA pairs.  A and B scale
 // buffers are viewed as rows of 256 bytes (half a 512-byte atom): one K step of one 128-row tile
 // is 8 consecutive rows.
-template <bool kSwiglu>
+template <int kMode>
 int launch_two_sm(GemmArgs& g, const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmO,
                   const void* a_scale, int64_t a_rows, const void* b_scale, int64_t b_rows, int clusters_wanted,
-                  int dev, cudaStream_t st, const CUtensorMap* tmH = nullptr) {
+                  int dev, cudaStream_t st, const CUtensorMap* tmH = nullptr, const CUtensorMap* tmR = nullptr) {
   CUtensorMap tmSA, tmSB;
   if (!rb_host::make_tmap_2d(&tmSA, a_scale, CU_TENSOR_MAP_DATA_TYPE_UINT8, 256,
                              (uint64_t)(a_rows / 128) * (uint64_t)g.kb_total * 2, 256, 256, 8,
@@ -1187,7 +1411,7 @@ int launch_two_sm(GemmArgs& g, const CUtensorMap& tmA, const CUtensorMap& tmB, c
                              CU_TENSOR_MAP_SWIZZLE_NONE))
     return RB_ERR_CUDA;
   const int sms = rb_host::sm_budget(dev);
-  const size_t smem = sizeof(Gemm2Smem<kSwiglu>) + 1024;
+  const size_t smem = sizeof(Gemm2Smem<kMode>) + 1024;
   static int max_clusters[64] = {0};
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -1195,20 +1419,20 @@ int launch_two_sm(GemmArgs& g, const CUtensorMap& tmA, const CUtensorMap& tmB, c
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(Gemm2Cfg<kSwiglu>::kThreads, 1, 1);
+  cfg.blockDim = dim3(Gemm2Cfg<kMode>::kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (dev >= 0 && dev < 64 && max_clusters[dev] == 0) {
-    if (cudaFuncSetAttribute(nvfp4_gemm2_kernel<kSwiglu>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+    if (cudaFuncSetAttribute(nvfp4_gemm2_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
         cudaSuccess) {
       rb_host::set_error("cudaFuncSetAttribute(gemm2) failed: %s", cudaGetErrorString(cudaGetLastError()));
       return RB_ERR_CUDA;
     }
     cfg.gridDim = dim3(2 * (sms / 2), 1, 1);
     int nc = 0;
-    if (cudaOccupancyMaxActiveClusters(&nc, nvfp4_gemm2_kernel<kSwiglu>, &cfg) != cudaSuccess || nc < 1) {
+    if (cudaOccupancyMaxActiveClusters(&nc, nvfp4_gemm2_kernel<kMode>, &cfg) != cudaSuccess || nc < 1) {
       cudaGetLastError();
       nc = sms / 2;
     }
@@ -1218,9 +1442,10 @@ int launch_two_sm(GemmArgs& g, const CUtensorMap& tmA, const CUtensorMap& tmB, c
   const int clusters = clusters_wanted < cap ? clusters_wanted : cap;
   if (clusters < 1) return RB_OK;
   cfg.gridDim = dim3(2 * clusters, 1, 1);
-  // tmH (SwiGLU mode: the h output) is unused by the plain kernel, which gets tmO in its place.
-  cudaError_t e = cudaLaunchKernelEx(&cfg, nvfp4_gemm2_kernel<kSwiglu>, tmA, tmB, tmSA, tmSB, tmO,
-                                     tmH != nullptr ? *tmH : tmO, g);
+  // A kernel that does not use tmH (SwiGLU mode: the h output; fused mode: the pre-activations) or tmR
+  // (fused mode: the residual) gets tmO in its place.
+  cudaError_t e = cudaLaunchKernelEx(&cfg, nvfp4_gemm2_kernel<kMode>, tmA, tmB, tmSA, tmSB, tmO,
+                                     tmH != nullptr ? *tmH : tmO, tmR != nullptr ? *tmR : tmO, g);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {
     rb_host::set_error("nvfp4 gemm launch failed: %s", cudaGetErrorString(e));
@@ -1317,10 +1542,22 @@ struct SwigluOut {
   float* gs = nullptr;
 };
 
+// The fused epilogue of rb_nvfp4_gemm_epilogue (off for the other GEMMs).
+struct FusedEpilogue {
+  bool on = false;
+  int act = RB_ACT_NONE;
+  double p = 0.0;
+  const int64_t* seed = nullptr;
+  const void* residual = nullptr;
+  int64_t ldr = 0;
+  void* preact = nullptr;
+  int64_t ldz = 0;
+};
+
 static int gemm_impl(const void* a_packed, const void* a_scale, const void* b_packed, const void* b_scale, int64_t m,
                      int64_t n, int64_t k, const float* alpha_a, const float* alpha_b, const void* bias,
                      int bias_dtype, void* out, int out_dtype, int64_t ldo, void* const* peer_out, int npeers,
-                     void* stream, const SwigluOut& sw = SwigluOut()) {
+                     void* stream, const SwigluOut& sw = SwigluOut(), const FusedEpilogue& fe = FusedEpilogue()) {
   if (npeers < 0 || npeers > kMaxPeers || (npeers > 0 && peer_out == nullptr)) {
     rb_host::set_error("nvfp4 gemm: npeers must be in [0, %d] with a peer pointer array", kMaxPeers);
     return RB_ERR_ARG;
@@ -1363,9 +1600,29 @@ static int gemm_impl(const void* a_packed, const void* a_scale, const void* b_pa
                        "and a 16-byte row stride, an 8-byte aligned zeroed workspace and a global-scale pointer");
     return RB_ERR_ARG;
   }
+  if (fe.on) {
+    if (fe.act < RB_ACT_NONE || fe.act > RB_ACT_GELU_TANH || !(fe.p >= 0.0 && fe.p <= 1.0) ||
+        (fe.p > 0.0 && (fe.seed == nullptr || (reinterpret_cast<uintptr_t>(fe.seed) & 7) != 0))) {
+      rb_host::set_error("nvfp4 gemm_epilogue: needs a known activation (got %d), a dropout probability in [0, 1] "
+                         "(got %g) and with dropout an 8-byte aligned device seed", fe.act, fe.p);
+      return RB_ERR_ARG;
+    }
+    const auto bad = [&](const void* t, int64_t ld) {
+      return t != nullptr && (misaligned(t) || ld < n || ((uint64_t)ld * oesize) % 16 != 0);
+    };
+    if (bad(fe.residual, fe.ldr) || bad(fe.preact, fe.ldz)) {
+      rb_host::set_error("nvfp4 gemm_epilogue: residual and pre-activations must be 16-byte aligned with 16-byte row "
+                         "strides of at least n elements");
+      return RB_ERR_ARG;
+    }
+  }
   int dev = rb_host::current_device();
   if (!sm100_device(dev, "nvfp4 gemm")) return RB_ERR_DEVICE;
   GemmArgs g;
+  g.act = fe.act;
+  g.has_residual = fe.residual != nullptr;
+  g.has_preact = fe.preact != nullptr;
+  g.drop = rb_host::dropout_args(fe.p, fe.seed);
   g.h = sw.h;
   g.ldh = sw.ldh;
   g.h_ws = sw.ws;
@@ -1393,7 +1650,7 @@ static int gemm_impl(const void* a_packed, const void* a_scale, const void* b_pa
   g.tiles_n = (int)((n + kBN - 1) / kBN);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int sms = rb_host::sm_budget(dev);
-  const bool two_sm = m >= 256;
+  const bool two_sm = m >= 256 || fe.on;  // the fused epilogue exists on CTA pairs (half idle at m = 128)
   CUtensorMap tmA, tmB, tmO;
   // Output boxes are 32 rows x 128 bytes (64 bf16 or 32 fp32 columns), 128-byte swizzled.
   if (!rb_host::make_tmap_2d(&tmA, a_packed, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)(k / 2), (uint64_t)m,
@@ -1407,15 +1664,28 @@ static int gemm_impl(const void* a_packed, const void* a_scale, const void* b_pa
   if (two_sm) {
     g.tiles_m = (int)((m + 255) / 256);
     g.n_tiles = g.tiles_m * g.tiles_n;
+    if (fe.on) {
+      const auto dt = oesize == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+      CUtensorMap tmZ, tmR;
+      if ((fe.preact != nullptr && !rb_host::make_tmap_2d(&tmZ, fe.preact, dt, (uint64_t)n, (uint64_t)m,
+                                                          (uint64_t)fe.ldz * oesize, 128 / oesize, 32,
+                                                          CU_TENSOR_MAP_SWIZZLE_128B)) ||
+          (fe.residual != nullptr && !rb_host::make_tmap_2d(&tmR, fe.residual, dt, (uint64_t)n, (uint64_t)m,
+                                                            (uint64_t)fe.ldr * oesize, 128 / oesize, 32,
+                                                            CU_TENSOR_MAP_SWIZZLE_128B)))
+        return RB_ERR_CUDA;
+      return launch_two_sm<kFused>(g, tmA, tmB, tmO, a_scale, m, b_scale, n, g.n_tiles, dev, st,
+                                   fe.preact != nullptr ? &tmZ : nullptr, fe.residual != nullptr ? &tmR : nullptr);
+    }
     if (swiglu) {
       // h boxes: 32 rows x 32 bf16 (64 bytes), 64-byte swizzled; rows past m are clipped.
       CUtensorMap tmH;
       if (!rb_host::make_tmap_2d(&tmH, sw.h, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (uint64_t)(n / 2), (uint64_t)m,
                                  (uint64_t)sw.ldh * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
         return RB_ERR_CUDA;
-      return launch_two_sm<true>(g, tmA, tmB, tmO, a_scale, m, b_scale, n, g.n_tiles, dev, st, &tmH);
+      return launch_two_sm<kSwigluMode>(g, tmA, tmB, tmO, a_scale, m, b_scale, n, g.n_tiles, dev, st, &tmH);
     }
-    return launch_two_sm<false>(g, tmA, tmB, tmO, a_scale, m, b_scale, n, g.n_tiles, dev, st);
+    return launch_two_sm<kPlain>(g, tmA, tmB, tmO, a_scale, m, b_scale, n, g.n_tiles, dev, st);
   }
   g.tiles_m = (int)(m / kBM);
   g.n_tiles = g.tiles_m * g.tiles_n;
@@ -1452,6 +1722,24 @@ int rb_nvfp4_gemm_swiglu(const void* a_packed, const void* a_scale, const void* 
   sw.gs = h_global_scale;
   return gemm_impl(a_packed, a_scale, b_packed, b_scale, m, n, k, alpha_a, alpha_b, bias, bias_dtype, out,
                    RB_OUT_BF16, ldo, nullptr, 0, stream, sw);
+}
+
+int rb_nvfp4_gemm_epilogue(const void* a_packed, const void* a_scale, const void* b_packed, const void* b_scale,
+                           int64_t m, int64_t n, int64_t k, const float* alpha_a, const float* alpha_b,
+                           const void* bias, int bias_dtype, int activation, double p, const int64_t* seed,
+                           const void* residual, int64_t ldr, void* preact, int64_t ldz, void* out, int out_dtype,
+                           int64_t ldo, void* stream) {
+  FusedEpilogue fe;
+  fe.on = true;
+  fe.act = activation;
+  fe.p = p;
+  fe.seed = seed;
+  fe.residual = residual;
+  fe.ldr = ldr;
+  fe.preact = preact;
+  fe.ldz = ldz;
+  return gemm_impl(a_packed, a_scale, b_packed, b_scale, m, n, k, alpha_a, alpha_b, bias, bias_dtype, out, out_dtype,
+                   ldo, nullptr, 0, stream, SwigluOut(), fe);
 }
 
 int rb_nvfp4_selftest_silu(uint32_t* mismatches, void* stream) {
@@ -1511,6 +1799,9 @@ int rb_nvfp4_gemm_grouped(const void* a_packed, const void* a_scale, int64_t a_r
   int dev = rb_host::current_device();
   if (!sm100_device(dev, "nvfp4 grouped gemm")) return RB_ERR_DEVICE;
   GemmArgs g;
+  g.act = RB_ACT_NONE;
+  g.has_residual = g.has_preact = 0;
+  g.drop = rb_host::dropout_args(0.0, nullptr);
   g.h = nullptr;
   g.ldh = 0;
   g.h_ws = nullptr;
@@ -1549,8 +1840,8 @@ int rb_nvfp4_gemm_grouped(const void* a_packed, const void* a_scale, int64_t a_r
     return RB_ERR_CUDA;
   // The group sizes live on the device: every resident cluster starts, reads the table and takes
   // its share of the tiles (clusters without one exit).
-  return launch_two_sm<false>(g, tmA, tmB, tmO, a_scale, a_rows, b_scale, b_rows, 1 << 30, dev,
-                       reinterpret_cast<cudaStream_t>(stream));
+  return launch_two_sm<kPlain>(g, tmA, tmB, tmO, a_scale, a_rows, b_scale, b_rows, 1 << 30, dev,
+                               reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -17,7 +17,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import _trace
-from .quantize import _require_cuda, _stream_ptr
+from .quantize import NVFP4Tensor, _require_cuda, _stream_ptr
 
 _DTYPES = {torch.bfloat16: _lib.RB_DTYPE_BF16, torch.float32: _lib.RB_DTYPE_F32}
 
@@ -142,7 +142,7 @@ def dropout(x: torch.Tensor, p: float = 0.5, *, seed: torch.Tensor | int | None 
 
 
 # ------------------------------------------------------------------------------------------------
-# The backward of the GEMM epilogue
+# The GEMM with its sublayer's end, and the backward of that end
 # ------------------------------------------------------------------------------------------------
 
 
@@ -152,6 +152,83 @@ def _activation_code(activation: str | None, what: str) -> int:
         names = ", ".join(repr(a) for a in _lib.RB_ACTIVATIONS)
         raise ValueError(f"{what}: activation must be one of {names}, got {activation!r}")
     return code
+
+
+def _tma_rows(x: torch.Tensor) -> torch.Tensor:
+    """A 2-D tensor that a TMA tensor map can describe: 16-byte aligned, with 16-byte row strides."""
+    x, ld = _rows(x)
+    return x if x.data_ptr() % 16 == 0 and ld * x.element_size() % 16 == 0 else x.contiguous().clone()
+
+
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two 2-D tensors of one shape and dtype, with contiguous rows, share an element; rows of
+    one stride may interleave (column slices of one buffer)."""
+    size, (rows, cols) = a.element_size(), a.shape
+    lda, ldb = _rows(a)[1] * size, _rows(b)[1] * size
+    width, pa, pb = cols * size, a.data_ptr(), b.data_ptr()
+    if pa + (rows - 1) * lda + width <= pb or pb + (rows - 1) * ldb + width <= pa:
+        return False
+    at = (pb - pa) % lda
+    return lda != ldb or at < width or at + width > lda
+
+
+def epilogue_mm(a: NVFP4Tensor, b: NVFP4Tensor, *, bias: torch.Tensor | None = None, activation: str | None = None,
+                dropout_p: float = 0.0, seed: torch.Tensor | int | None = None, residual: torch.Tensor | None = None,
+                out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None, save_preact: bool = False
+                ) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """``residual + drop(act(z))`` with ``z = (a @ b.T) * (ga * gb) + bias``, in one GEMM.
+
+    ``mm`` with the end of a sublayer in its epilogue: everything after the accumulator is fp32 and is
+    rounded once, to ``out_dtype`` (bf16 or fp32).  ``activation``: None, "relu", "relu2", "silu", "gelu"
+    (erf) or "gelu_tanh".  ``dropout_p`` and ``seed`` as in ``dropout`` (None: a fresh seed; a backward
+    pass needs the seed, so keep it).  ``residual``: ``(M, N)`` of ``out_dtype``.  ``out`` may be the
+    residual itself.  With ``save_preact`` also returns ``z`` in ``out_dtype``, which
+    ``epilogue_backward`` takes.
+    """
+    what = "nvfp4.epilogue_mm"
+    _require_cuda(a.packed, what)
+    dev = a.packed.device
+    ap, asc = a.packed.view(torch.uint8), a.scale.view(torch.uint8)
+    bp, bsc = b.packed.view(torch.uint8), b.scale.view(torch.uint8)
+    (m, k2), (n, k2b) = ap.shape, bp.shape
+    if k2 != k2b:
+        raise ValueError(f"{what}: contraction mismatch {2 * k2} vs {2 * k2b}")
+    if out_dtype not in _DTYPES:
+        raise ValueError(f"{what}: unsupported output dtype {out_dtype} (bf16 or fp32)")
+    act, p = _activation_code(activation, what), _probability(dropout_p, what)
+    seed = _seed_tensor(seed, dev, what) if p > 0.0 else None
+    bias_code = 0
+    if bias is not None:
+        if bias.shape != (n,) or bias.device != dev:
+            raise ValueError(f"{what}: bias must have shape ({n},) on {dev}, got {tuple(bias.shape)} on {bias.device}")
+        if bias.dtype not in _DTYPES:
+            bias = bias.to(torch.float32)
+        bias = bias.contiguous()
+        if bias.data_ptr() % 16:  # the epilogue reads the bias in 16-byte vectors
+            bias = bias.clone()
+        bias_code = _DTYPES[bias.dtype]
+    if residual is not None:
+        _like("residual", residual, (m, n), out_dtype, dev, what)
+    if out is None:
+        out = torch.empty(m, n, dtype=out_dtype, device=dev)
+    else:
+        _like("out", out, (m, n), out_dtype, dev, what)
+        if _tma_rows(out) is not out:
+            raise ValueError(f"{what}: out must be 16-byte aligned with contiguous rows and 16-byte row strides")
+        if residual is not None and _share_memory(out, _rows(residual)[0]) and not (
+                out.data_ptr() == residual.data_ptr() and out.stride() == residual.stride()):
+            raise ValueError(f"{what}: out overlaps the residual without being the residual")
+    if residual is not None:
+        residual = _tma_rows(residual)
+    z = torch.empty(m, n, dtype=out_dtype, device=dev) if save_preact else None
+    tok = _trace.begin("gemm", 4.0 * m * n * k2)
+    _call(what, dev, _lib.load().rb_nvfp4_gemm_epilogue, ap.data_ptr(), asc.data_ptr(), bp.data_ptr(), bsc.data_ptr(),
+          m, n, 2 * k2, a.global_scale.data_ptr(), b.global_scale.data_ptr(), None if bias is None else bias.data_ptr(),
+          bias_code, act, p, None if seed is None else seed.data_ptr(),
+          None if residual is None else residual.data_ptr(), n if residual is None else _rows(residual)[1],
+          None if z is None else z.data_ptr(), n, out.data_ptr(), _DTYPES[out_dtype], _rows(out)[1])
+    _trace.end(tok)
+    return (out, z) if save_preact else out
 
 
 def epilogue_backward(grad_y: torch.Tensor, preact: torch.Tensor | None = None, *, activation: str | None = None,

@@ -45,6 +45,7 @@ from .quantize import (
     row_scale_bytes,
     swiglu,
 )
+from .routing import Routing, route, token_combine, token_dispatch
 
 ALIGN = 128
 
@@ -435,6 +436,38 @@ class FP4BatchedExperts(nn.Module):
 
     def forward_sorted(self, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
         return self.down(swiglu(self.gate_up(x, offsets), "split"), offsets)
+
+    def forward_routed(self, x: torch.Tensor, logits: torch.Tensor, k: int, *,
+                       expert_bias: torch.Tensor | None = None, valid: torch.Tensor | None = None,
+                       renormalize: bool = True, residual: torch.Tensor | None = None
+                       ) -> tuple[torch.Tensor, Routing]:
+        """The whole mixture-of-experts sublayer on tokens ``(..., d_model)`` with router logits
+        ``(..., n_experts)``: ``residual + sum_j w_j expert_j(x)`` over each token's top ``k`` experts
+        (``MoEFeedForward``, ffn.py:156-436, without a capacity: no token is dropped), and the
+        ``Routing`` with its balance loss and counts.  Rows go to the experts and back with
+        ``token_dispatch`` and ``token_combine``; ``valid`` masks padding tokens (bool, the leading shape)."""
+        d, e = self.d_model, self.n_experts
+        if x.shape[-1] != d or logits.shape != (*x.shape[:-1], e):
+            raise ValueError(f"FP4BatchedExperts.forward_routed: expected tokens (..., {d}) and logits (..., {e}), got "
+                             f"{tuple(x.shape)} and {tuple(logits.shape)}")
+        routing = route(logits.reshape(-1, e), k, expert_bias=expert_bias,
+                        valid=None if valid is None else valid.reshape(-1), renormalize=renormalize)
+        if routing.num_rows == 0:  # no tokens
+            return (torch.zeros_like(x) if residual is None else residual.clone()), routing
+        xs = token_dispatch(x.reshape(-1, d), routing)
+        # Biases: (rows x experts) one-hot times the experts' biases.  What lies past the last group was never
+        # written, in the linears' outputs and in their input gradients alike; the bias gradient sums over
+        # all rows, so both are cut to 0 there.
+        start = routing.offsets[:-1]
+        row = torch.arange(routing.num_rows, device=x.device).unsqueeze(1)
+        hot = ((row >= start) & (row < start + routing.counts)).to(xs.dtype)
+        h = torch.addmm(self.gate_up(xs, routing.offsets), hot, self.gate_up_b.squeeze(1).to(xs.dtype))
+        h = torch.where(row < routing.offsets[-1], h, 0)
+        y = self.down(swiglu(h, "split"), routing.offsets)
+        y = torch.addmm(y, hot, self.down_b.squeeze(1).to(y.dtype))
+        if residual is not None:
+            residual = residual.reshape(-1, d)
+        return token_combine(y, routing, residual=residual).view(x.shape), routing
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         e, cap, d = x.shape

@@ -21,6 +21,16 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .epilogue import (
+    _activation_code,
+    _dtype_of,
+    _like,
+    _probability,
+    _seed_tensor,
+    dropout,
+    epilogue_backward,
+    epilogue_mm,
+)
 from .quantize import (
     BLOCK,
     NVFP4Tensor,
@@ -66,7 +76,7 @@ class _FP4LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, w_fwd_packed, w_fwd_scale, w_fwd_gs, w_dgrad_packed, w_dgrad_scale,
                 w_dgrad_gs, hadamard, seed, recipe, reduce_grad_scale=None, output_gemm=None, x_global_scale=None,
-                wgrad_hook=None):
+                wgrad_hook=None, also_saved=()):
         # The input's global scale comes from its producer when that computed it (a SwiGLU epilogue);
         # otherwise the quantizer computes it in the same launch (global_scale_of, linear.py:79).
         rot = hadamard if recipe.hadamard and hadamard.numel() else None
@@ -88,7 +98,7 @@ class _FP4LinearFn(torch.autograd.Function):
             saved = (xqt.packed, xqt.scale, weight, w_dgrad_packed, w_dgrad_scale, w_dgrad_gs, hadamard, seed, gx)
         else:
             saved = (x, x, weight, w_dgrad_packed, w_dgrad_scale, w_dgrad_gs, hadamard, seed, gx)
-        ctx.save_for_backward(*saved)
+        ctx.save_for_backward(*saved, *also_saved)  # what output_gemm left for its own backward comes last
         ctx.recipe = recipe
         ctx.reduce_grad_scale = reduce_grad_scale
         ctx.wgrad_hook = wgrad_hook
@@ -100,7 +110,7 @@ class _FP4LinearFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_y):
-        xt_or_x, xt_scale, weight, wt_packed, wt_scale, wt_gs, hadamard, seed, gx = ctx.saved_tensors
+        xt_or_x, xt_scale, weight, wt_packed, wt_scale, wt_gs, hadamard, seed, gx = ctx.saved_tensors[:9]
         recipe: FP4Recipe = ctx.recipe
         if grad_y.stride(-1) != 1:  # row-strided gradients (an N-split slice) are read in place
             grad_y = grad_y.contiguous()
@@ -108,10 +118,11 @@ class _FP4LinearFn(torch.autograd.Function):
         fp4_backward = recipe.grad_gemms and quantize_supported_shape(*grad_y.shape)
         if fp4_backward:
             rot = hadamard if recipe.hadamard and hadamard.numel() else None
-            # dY's global scale: from its producer when that computed it (the SwiGLU backward), else
-            # computed by the quantizer in the same launch.
+            # dY's global scale: from its producer when that computed it (the SwiGLU or epilogue
+            # backward), else computed by the quantizer in the same launch.
             gg = getattr(ctx, "grad_global_scale", None)
-            if ctx.has_bias:  # the bias gradient's column sums come from the same read of dY
+            colsum = getattr(ctx, "grad_column_sums", None)
+            if ctx.has_bias and colsum is None:  # the bias gradient's column sums come from the same read of dY
                 gg, colsum = global_scale_and_column_sums(grad_y)
             elif ctx.reduce_grad_scale is not None and gg is None:
                 gg = global_scale_of(grad_y)
@@ -143,6 +154,50 @@ class _FP4LinearFn(torch.autograd.Function):
             None if grad_b is None else grad_b.to(weight.dtype),
             None, None, None, None, None, None, None, None, None, None, None, None, None,
         )
+
+
+class _FP4EpilogueLinearFn(torch.autograd.Function):
+    """``residual + drop(act(x W^T + b))``: ``_FP4LinearFn`` with the output GEMM replaced by
+    ``epilogue_mm``.  The backward of what follows the product is one kernel (``epilogue_backward``), which
+    also hands the linear's backward its gradient's global scale and the bias gradient; the residual's
+    gradient is the upstream one.  The pre-activations are kept for an activation, the dropout mask never."""
+
+    @staticmethod
+    def forward(ctx, residual, activation, dropout_p, dropout_seed, x, *args):
+        extra = []
+
+        def gemm(xq, wq, b, out_dtype):
+            keep = activation is not None
+            y = epilogue_mm(xq, wq, bias=b, activation=activation, dropout_p=dropout_p, seed=dropout_seed,
+                            residual=residual, out_dtype=out_dtype, save_preact=keep)
+            y, z = y if keep else (y, None)
+            extra.extend((z, dropout_seed))
+            return y
+
+        # args: weight .. reduce_grad_scale (12), the input's global scale, the wgrad hook
+        y = _FP4LinearFn.forward(ctx, x, *args[:12], gemm, args[12], args[13], extra)
+        ctx.activation, ctx.dropout_p = activation, dropout_p
+        return y
+
+    @staticmethod
+    def backward(ctx, grad_y):
+        z, seed = ctx.saved_tensors[9:]
+        grad_z = grad_y
+        if ctx.activation is not None or ctx.dropout_p > 0.0:
+            grad_z, ctx.grad_global_scale, ctx.grad_column_sums = epilogue_backward(
+                grad_y, z, activation=ctx.activation, dropout_p=ctx.dropout_p, seed=seed, bias_grad=ctx.has_bias)
+        grads = _FP4LinearFn.backward(ctx, grad_z)
+        return (grad_y if ctx.needs_input_grad[0] else None, None, None, None, *grads[:13], *grads[14:16])
+
+
+_TORCH_ACTIVATIONS = {
+    None: lambda z: z,
+    "relu": F.relu,
+    "relu2": lambda z: F.relu(z).square(),
+    "silu": F.silu,
+    "gelu": F.gelu,
+    "gelu_tanh": lambda z: F.gelu(z, approximate="tanh"),
+}
 
 
 class FP4Linear(nn.Linear):
@@ -241,16 +296,47 @@ class FP4Linear(nn.Linear):
             self._hadamard, self._seed, self.recipe, self.reduce_grad_scale,
         )
 
-    def forward(self, x: torch.Tensor, global_scale: torch.Tensor | None = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, global_scale: torch.Tensor | None = None, *, activation: str | None = None,
+                dropout_p: float = 0.0, dropout_seed: torch.Tensor | int | None = None,
+                residual: torch.Tensor | None = None) -> torch.Tensor:
         """``global_scale``: the input's 0-d fp32 global scale when its producer has computed it
-        (``FP4SwiGLU``); by default the layer computes it (linear.py:79)."""
+        (``FP4SwiGLU``); by default the layer computes it (linear.py:79).
+
+        With ``activation`` (``epilogue_mm``'s names), ``dropout_p`` or ``residual`` (the output's shape, the
+        input's dtype) the layer returns ``residual + drop(act(x W^T + b))`` from the GEMM's epilogue.
+        Dropout is applied whenever ``dropout_p > 0``: pass 0 in evaluation.  ``dropout_seed``: as ``dropout``'s
+        ``seed``.  On the bf16 fallback path the same ops run one after the other."""
         self._check_device(x)
+        plain = activation is None and dropout_p == 0.0 and residual is None
+        if not plain:
+            self._check_epilogue(x, activation, dropout_p, residual)
         if not self._eligible(x):
             _warn_fallback_once(self, x)
-            return F.linear(x, self.weight.to(x.dtype), None if self.bias is None else self.bias.to(x.dtype))
+            y = F.linear(x, self.weight.to(x.dtype), None if self.bias is None else self.bias.to(x.dtype))
+            if plain:
+                return y
+            y = _TORCH_ACTIVATIONS[activation](y)
+            return dropout(y, dropout_p, seed=dropout_seed, residual=residual)
         flat = x.reshape(-1, self.in_features).contiguous()
-        y = _FP4LinearFn.apply(*self._fn_args(flat), self.output_gemm, global_scale, self.wgrad_hook)
+        if plain:
+            y = _FP4LinearFn.apply(*self._fn_args(flat), self.output_gemm, global_scale, self.wgrad_hook)
+        else:
+            seed = _seed_tensor(dropout_seed, x.device, type(self).__name__) if dropout_p > 0.0 else None
+            if residual is not None:
+                residual = residual.reshape(-1, self.out_features)
+            y = _FP4EpilogueLinearFn.apply(residual, activation, dropout_p, seed, *self._fn_args(flat), global_scale,
+                                           self.wgrad_hook)
         return y.view(*x.shape[:-1], self.out_features)
+
+    def _check_epilogue(self, x: torch.Tensor, activation, dropout_p, residual) -> None:
+        what = type(self).__name__
+        if self.output_gemm is not None:
+            raise ValueError(f"{what}: an N-split slice with a fused gather has no activation, dropout or residual")
+        _activation_code(activation, what)
+        _probability(dropout_p, what)
+        _dtype_of(x, what)
+        if residual is not None:
+            _like("residual", residual, (*x.shape[:-1], self.out_features), x.dtype, x.device, what)
 
 
 class _FP4SwiGLUFn(torch.autograd.Function):
@@ -363,8 +449,14 @@ class FP4FeedForward(nn.Module):
         mod.down_proj.invalidate_fp4_cache()
         return mod
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """``dropout(down_proj(...))``; with ``residual`` (the output's shape and dtype) the block's
+        ``residual + dropout(down_proj(...))`` from down_proj's epilogue, the mask drawn there (``dropout``'s
+        generator, seeded from torch's)."""
         h, gs = self.gate_up(x)
+        if residual is not None:
+            p = self.dropout.p if self.dropout.training else 0.0
+            return self.down_proj(h, global_scale=gs, dropout_p=p, residual=residual)
         return self.dropout(self.down_proj(h, global_scale=gs))
 
 

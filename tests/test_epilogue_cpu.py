@@ -68,6 +68,17 @@ def test_entry_points_refuse_on_the_host():
     assert lib.rb_nvfp4_dropout(buf, None, 0, -1, 0.0, None, buf, None) == 1
     assert lib.rb_nvfp4_dropout(None, None, 0, 0, 0.0, None, None, None) == 0  # nothing to do
 
+    def gemm(act=0, p=0.0, seed=None, res=None, ldr=128, z=None, ldz=128, out=buf, m=128, dt=0):
+        return lib.rb_nvfp4_gemm_epilogue(buf, buf, buf, buf, m, 128, 64, None, None, None, 0, act, p, seed, res, ldr,
+                                          z, ldz, out, dt, 128, None)
+
+    assert gemm(m=100) == 1 and "m % 128" in msg()
+    for kw in (dict(act=6), dict(act=-1), dict(p=1.5), dict(p=float("nan")), dict(p=0.5), dict(p=0.5, seed=odd)):
+        assert gemm(**kw) == 2 and "activation" in msg(), kw
+    for kw in (dict(res=odd), dict(res=buf, ldr=127), dict(res=buf, ldr=132), dict(z=odd), dict(z=buf, ldz=64)):
+        assert gemm(**kw) == 2 and "residual" in msg(), kw
+    assert gemm(out=None) == 2 and gemm(dt=5) == 2
+
     def back(rows=4, cols=8, ldg=8, z=buf, act=4, ws=buf, out=buf, p=0.0, seed=None):
         return lib.rb_nvfp4_epilogue_backward(buf, ldg, z, 8, 0, rows, cols, act, p, seed, out, 8, buf, None, ws,
                                               1 << 20, None)
@@ -112,7 +123,8 @@ def test_operators_refuse_cpu_tensors():
     x = torch.randn(128, 64)
     r = nv.Routing(torch.zeros(128, 2), torch.zeros(128, 2, dtype=torch.int32), torch.zeros(4, dtype=torch.int64),
                    torch.zeros(()), torch.zeros(5, dtype=torch.int64), torch.zeros(128, 2, dtype=torch.int32), 512)
-    for call in (lambda: nv.dropout(x, 0.5), lambda: nv.epilogue_backward(x), lambda: nv.route(x, 2),
+    q = nv.NVFP4Tensor(torch.zeros(128, 32, dtype=torch.uint8), torch.zeros(1024, dtype=torch.uint8), torch.ones(()))
+    for call in (lambda: nv.dropout(x, 0.5), lambda: nv.epilogue_mm(q, q), lambda: nv.epilogue_backward(x), lambda: nv.route(x, 2),
                  lambda: nv.token_dispatch(x, r), lambda: nv.token_combine(x, r)):
         with pytest.raises(RuntimeError, match="no CPU"):
             call()
