@@ -17,31 +17,27 @@ namespace rb {
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* x, const T* residual, T* y, int64_t n,
                                                       const DropoutArgs d) {
-  const PhiloxKey key = d.seed != nullptr ? philox_key(d.seed) : PhiloxKey{0, 0};
+  const PhiloxKeys key = philox_keys<true>(d.seed);
   const int64_t groups = (n + 7) / 8, step = (int64_t)gridDim.x * blockDim.x;
   for (int64_t g = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; g < groups; g += step) {
     const int64_t i = 8 * g;
-    float v[8];
+    float2 v[4];
     if (kVec && i + 8 <= n) {
+      float2 r[4];
       Io<T>::load8(v, x + i);
+      if (residual != nullptr) Io<T>::load8(r, residual + i);
+      if (d.seed != nullptr) dropout8(v, (uint64_t)g, key, d.below, d.scale);
       if (residual != nullptr) {
-        float r[8];
-        Io<T>::load8(r, residual + i);
-        if (d.seed != nullptr) dropout8(v, (uint64_t)g, key, d.threshold, d.scale);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += r[j];
-      } else if (d.seed != nullptr) {
-        dropout8(v, (uint64_t)g, key, d.threshold, d.scale);
+        for (int j = 0; j < 4; ++j) v[j] = __fadd2_rn(v[j], r[j]);
       }
       Io<T>::store8(y + i, v);
     } else {
-      const int m = (int)min((int64_t)8, n - i);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < m ? Io<T>::load(x + i + j) : 0.0f;
-      if (d.seed != nullptr) dropout8(v, (uint64_t)g, key, d.threshold, d.scale);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < m) Io<T>::store(y + i + j, residual != nullptr ? v[j] + Io<T>::load(residual + i + j) : v[j]);
+      for (int j = 0; j < 8 && i + j < n; ++j) {
+        float u = Io<T>::load(x + i + j);
+        if (d.seed != nullptr) u = dropout1(u, (uint64_t)(i + j), key, d.below, d.scale);
+        Io<T>::store(y + i + j, residual != nullptr ? u + Io<T>::load(residual + i + j) : u);
+      }
     }
   }
 }
@@ -64,46 +60,45 @@ constexpr int kBwdLanes = 32;  // threads along a row, 8 columns each: a block c
 constexpr int kBwdRows = 8;    // rows a block reads at once
 
 template <typename T, int kAct, bool kVec>
-__global__ void __launch_bounds__(kBwdLanes* kBwdRows) epilogue_backward_kernel(const EpilogueBwdArgs a) {
+__global__ void __launch_bounds__(kBwdLanes* kBwdRows, kVec ? 4 : 2) epilogue_backward_kernel(const EpilogueBwdArgs a) {
   const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t c = ((int64_t)blockIdx.x * kBwdLanes + lane) * 8;
   const int64_t r0 = (int64_t)blockIdx.y * a.rows_per_block, r1 = min(a.rows, r0 + a.rows_per_block);
-  const PhiloxKey key = a.drop.seed != nullptr ? philox_key(a.drop.seed) : PhiloxKey{0, 0};
   const T* dy = reinterpret_cast<const T*>(a.dy);
   const T* z = reinterpret_cast<const T*>(a.z);
   T* dz = reinterpret_cast<T*>(a.dz);
-  float sum[8];
+  float2 sum[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sum[j] = 0.0f;
+  for (int j = 0; j < 4; ++j) sum[j] = both(0.0f);
   uint32_t m = 0;
   if (c < a.cols) {
-#pragma unroll (kVec ? 2 : 1)
-    for (int64_t r = r0 + ty; r < r1; r += kBwdRows) {
-      float g[8];
-      if constexpr (kVec) {
-        float zv[8];
+    const PhiloxKeys key = philox_keys<false>(a.drop.seed);
+    if constexpr (kVec) {
+#pragma unroll 2
+      for (int64_t r = r0 + ty; r < r1; r += kBwdRows) {
+        float2 g[4], zv[4];
         Io<T>::load8(g, dy + r * a.ldg + c);
         if constexpr (kAct != RB_ACT_NONE) Io<T>::load8(zv, z + r * a.ldz + c);
-        if (a.drop.seed != nullptr)
-          dropout8(g, (uint64_t)(r * a.cols + c) >> 3, key, a.drop.threshold, a.drop.scale);
+        if (a.drop.seed != nullptr) dropout8(g, (uint64_t)(r * a.cols + c) >> 3, key, a.drop.below, a.drop.scale);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if constexpr (kAct != RB_ACT_NONE) g[j] *= act_derivative<kAct>(zv[j]);
-          sum[j] += g[j];
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (kAct != RB_ACT_NONE) g[j] = __fmul2_rn(g[j], act_derivative2<kAct>(zv[j]));
+          sum[j] = __fadd2_rn(sum[j], g[j]);
         }
-        Io<T>::store8(dz + r * a.ldo + c, g);  // g becomes the rounded values
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(g[j]) & 0x7FFFFFFFu);
-      } else {
+        m = max(m, Io<T>::store8(dz + r * a.ldo + c, g));
+      }
+    } else {
+      for (int64_t r = r0 + ty; r < r1; r += kBwdRows) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (c + j >= a.cols) break;
           float v = Io<T>::load(dy + r * a.ldg + c + j);
           if (a.drop.seed != nullptr)
-            v = dropout1(v, (uint64_t)(r * a.cols + c + j), key, a.drop.threshold, a.drop.scale);
-          if constexpr (kAct != RB_ACT_NONE) v *= act_derivative<kAct>(Io<T>::load(z + r * a.ldz + c + j));
-          sum[j] += v;
-          m = max(m, __float_as_uint(Io<T>::store(dz + r * a.ldo + c + j, v)) & 0x7FFFFFFFu);
+            v = dropout1(v, (uint64_t)(r * a.cols + c + j), key, a.drop.below, a.drop.scale);
+          if constexpr (kAct != RB_ACT_NONE) v *= act_derivative2<kAct>(both(Io<T>::load(z + r * a.ldz + c + j))).x;
+          if (j & 1) sum[j / 2].y += v;
+          else sum[j / 2].x += v;
+          m = max(m, Io<T>::store(dz + r * a.ldo + c + j, v));
         }
       }
     }
@@ -115,7 +110,7 @@ __global__ void __launch_bounds__(kBwdLanes* kBwdRows) epilogue_backward_kernel(
   if (lane == 0) wmax[ty] = m;
   if (a.partial != nullptr) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) red[ty][j * 32 + lane] = sum[j];  // lanes on consecutive banks
+    for (int j = 0; j < 8; ++j) red[ty][j * 32 + lane] = (j & 1) ? sum[j / 2].y : sum[j / 2].x;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -220,10 +215,10 @@ int check_common(const char* what, int dtype, double p, const int64_t* seed) {
   return RB_OK;
 }
 
-// Row splits of the backward kernel: four blocks of 256 threads fit an SM beside one another, and
-// each gets at least 16 rows.
+// Row splits of the backward kernel: one wave of the four blocks that an SM holds at once (one block
+// more than that and the last ones run alone), each with at least 16 rows.
 int64_t backward_parts(int64_t rows, int64_t gx) {
-  const int64_t want = ((int64_t)4 * rb_host::sm_budget(rb_host::current_device()) + gx - 1) / gx;
+  const int64_t want = (int64_t)4 * rb_host::sm_budget(rb_host::current_device()) / gx;
   const int64_t most = (rows + 15) / 16;
   int64_t parts = want < most ? want : most;
   if (parts > 65535) parts = 65535;

@@ -22,91 +22,156 @@ namespace rb {
 // reciprocal of the probability that is really used, so the expectation is exact.
 struct DropoutArgs {
   const int64_t* seed;  // device; nullptr: no dropout
-  uint32_t threshold;   // 0 .. 65536
+  uint32_t below;       // threshold * 2^16 - 1: a draw in the upper half of a word stays when the word is above it
   float scale;
 };
 
-struct PhiloxKey {
-  uint32_t k0, k1;
+// The ten rounds' keys, which depend on the seed alone.  kHold: they are kept in 20 registers (the empty
+// asm hides that they could be computed again), sparing every call 18 additions, about a fifth of its
+// integer work; without it the compiler adds them up in each call.
+struct PhiloxKeys {
+  uint32_t k0[10], k1[10];
 };
 
-__device__ __forceinline__ PhiloxKey philox_key(const int64_t* seed) {
-  const uint64_t s = static_cast<uint64_t>(__ldg(reinterpret_cast<const long long*>(seed)));
-  return {static_cast<uint32_t>(s), static_cast<uint32_t>(s >> 32)};
+template <bool kHold>
+__device__ __forceinline__ PhiloxKeys philox_keys(const int64_t* seed) {
+  PhiloxKeys k;
+  const uint64_t s = seed != nullptr ? static_cast<uint64_t>(__ldg(reinterpret_cast<const long long*>(seed))) : 0;
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    k.k0[r] = static_cast<uint32_t>(s) + r * 0x9E3779B9u;
+    k.k1[r] = static_cast<uint32_t>(s >> 32) + r * 0xBB67AE85u;
+    if constexpr (kHold) asm("" : "+r"(k.k0[r]), "+r"(k.k1[r]));
+  }
+  return k;
 }
 
-__device__ __forceinline__ uint4 philox(uint64_t counter, PhiloxKey key) {
+__device__ __forceinline__ uint4 philox(uint64_t counter, const PhiloxKeys& key) {
   uint32_t c0 = static_cast<uint32_t>(counter), c1 = static_cast<uint32_t>(counter >> 32), c2 = 0, c3 = 0;
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t a = static_cast<uint64_t>(c0) * 0xD2511F53u, b = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
-    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ key.k0;
+    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ key.k0[r];
     c1 = static_cast<uint32_t>(b);
-    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ key.k1;
+    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ key.k1[r];
     c3 = static_cast<uint32_t>(a);
-    key.k0 += 0x9E3779B9u;
-    key.k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
 }
 
 // Drops from the eight elements 8 * group .. 8 * group + 7.  A dropped element is 0 whatever it
 // held, infinities and NaN included.
-__device__ __forceinline__ void dropout8(float (&v)[8], uint64_t group, PhiloxKey key, uint32_t threshold,
+__device__ __forceinline__ void dropout8(float2 (&v)[4], uint64_t group, const PhiloxKeys& key, uint32_t below,
                                          float scale) {
   const uint4 d = philox(group, key);
   const uint32_t w[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    v[2 * j] = (w[j] & 0xFFFFu) >= threshold ? v[2 * j] * scale : 0.0f;
-    v[2 * j + 1] = (w[j] >> 16) >= threshold ? v[2 * j + 1] * scale : 0.0f;
+    v[j].x = (w[j] << 16) > below ? v[j].x * scale : 0.0f;
+    v[j].y = w[j] > below ? v[j].y * scale : 0.0f;
   }
 }
 
 // One element, at any index.
-__device__ __forceinline__ float dropout1(float v, uint64_t index, PhiloxKey key, uint32_t threshold, float scale) {
+__device__ __forceinline__ float dropout1(float v, uint64_t index, const PhiloxKeys& key, uint32_t below,
+                                          float scale) {
   const uint4 d = philox(index >> 3, key);
   const uint32_t j = static_cast<uint32_t>(index) & 7u;
   const uint32_t lo = (j & 2) ? d.y : d.x, hi = (j & 2) ? d.w : d.z;
   const uint32_t w = (j & 4) ? hi : lo;
-  return ((j & 1) ? w >> 16 : w & 0xFFFFu) >= threshold ? v * scale : 0.0f;
+  return ((j & 1) ? w : w << 16) > below ? v * scale : 0.0f;
 }
 
 // ---------------------------------------------------------------------------------------------
-// Activations (RB_ACT_*)
+// Activations (RB_ACT_*), two elements at a time on the packed fp32 pipe
 // ---------------------------------------------------------------------------------------------
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + expf(-z)); }
+__device__ __forceinline__ float rcp_approx(float x) {  // within 1 ulp; inf -> 0
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float ex2_approx(float x) {  // within 2 ulp; large x -> inf, large -x -> 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 rcp2(float2 x) { return make_float2(rcp_approx(x.x), rcp_approx(x.y)); }
+__device__ __forceinline__ float2 ex2_2(float2 x) { return make_float2(ex2_approx(x.x), ex2_approx(x.y)); }
 
-constexpr float kSqrtHalf = 0.70710678118654752f;
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kGeluA = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluB = 0.044715f;
 
+__device__ __forceinline__ float2 sigmoid2(float2 z) {
+  return rcp2(__fadd2_rn(ex2_2(__fmul2_rn(z, both(-kLog2e))), both(1.0f)));
+}
+
 // 0.5 z (1 + tanh(u)) = z sigmoid(2u): one exponential, and no cancellation where tanh nears -1.
+__device__ __forceinline__ float2 gelu_tanh_sigmoid2(float2 z) {
+  const float2 w = __ffma2_rn(__fmul2_rn(z, z), both(-kLog2e * kGeluA * kGeluB), both(-kLog2e * kGeluA));
+  return rcp2(__fadd2_rn(ex2_2(__fmul2_rn(z, w)), both(1.0f)));
+}
+
+// The normal distribution's tail q = Phi(-|z|) = erfc(|z| / sqrt 2) / 2 and e = exp(-z^2 / 2), by
+// Hastings' formula (C. Hastings, "Approximations for Digital Computers", 1955, sheet 45; 7.1.26 of
+// Abramowitz and Stegun): erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), within
+// 1.5e-7 for x >= 0.  Halved here.  One reciprocal and one exponential, with e shared by the derivative, where
+// erff takes a branch and some 25 instructions more.  `az` is |z| held below 128, where q is 0.
+struct NormalTail {
+  float2 az, q, e;
+};
+__device__ __forceinline__ NormalTail normal_tail2(float2 z) {
+  NormalTail n;
+  n.az = make_float2(fminf(fabsf(z.x), 128.0f), fminf(fabsf(z.y), 128.0f));
+  const float2 t = rcp2(__ffma2_rn(n.az, both(0.3275911f * 0.70710678118654752f), both(1.0f)));
+  float2 p = __ffma2_rn(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+  p = __ffma2_rn(t, p, both(0.5f * 1.421413741f));
+  p = __ffma2_rn(t, p, both(0.5f * -0.284496736f));
+  p = __ffma2_rn(t, p, both(0.5f * 0.254829592f));
+  n.e = ex2_2(__fmul2_rn(z, __fmul2_rn(z, both(-0.5f * kLog2e))));
+  n.q = __fmul2_rn(__fmul2_rn(t, p), n.e);
+  return n;
+}
+
 template <int kAct>
-__device__ __forceinline__ float act_value(float z) {
-  if constexpr (kAct == RB_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN passes through
-  else if constexpr (kAct == RB_ACT_RELU2) return z < 0.0f ? 0.0f : z * z;
-  else if constexpr (kAct == RB_ACT_SILU) return z * sigmoid(z);
-  else if constexpr (kAct == RB_ACT_GELU) return 0.5f * z * (1.0f + erff(z * kSqrtHalf));
-  else if constexpr (kAct == RB_ACT_GELU_TANH) return z * sigmoid(kGeluA * fmaf(kGeluB * z * z, z, z));
+__device__ __forceinline__ float2 act_value2(float2 z) {
+  if constexpr (kAct == RB_ACT_RELU) return make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y);  // NaN stays
+  else if constexpr (kAct == RB_ACT_RELU2) {
+    const float2 r = make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y);
+    return __fmul2_rn(r, r);
+  } else if constexpr (kAct == RB_ACT_SILU) return __fmul2_rn(z, sigmoid2(z));
+  else if constexpr (kAct == RB_ACT_GELU) {
+    // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+    const NormalTail n = normal_tail2(z);
+    const float2 pos = make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y);
+    return __ffma2_rn(make_float2(-n.az.x, -n.az.y), n.q, pos);
+  } else if constexpr (kAct == RB_ACT_GELU_TANH) return __fmul2_rn(z, gelu_tanh_sigmoid2(z));
   else return z;
 }
 
 template <int kAct>
-__device__ __forceinline__ float act_derivative(float z) {
-  if constexpr (kAct == RB_ACT_RELU) return z <= 0.0f ? 0.0f : (z != z ? z : 1.0f);
-  else if constexpr (kAct == RB_ACT_RELU2) return z <= 0.0f ? 0.0f : 2.0f * z;
+__device__ __forceinline__ float2 act_derivative2(float2 z) {
+  if constexpr (kAct == RB_ACT_RELU)
+    return make_float2(z.x <= 0.0f ? 0.0f : (z.x != z.x ? z.x : 1.0f), z.y <= 0.0f ? 0.0f : (z.y != z.y ? z.y : 1.0f));
+  else if constexpr (kAct == RB_ACT_RELU2)
+    return make_float2(z.x <= 0.0f ? 0.0f : z.x + z.x, z.y <= 0.0f ? 0.0f : z.y + z.y);
   else if constexpr (kAct == RB_ACT_SILU) {
-    const float s = sigmoid(z);
-    return s * fmaf(z, 1.0f - s, 1.0f);
+    const float2 s = sigmoid2(z);
+    return __fmul2_rn(s, __ffma2_rn(z, __ffma2_rn(s, both(-1.0f), both(1.0f)), both(1.0f)));
   } else if constexpr (kAct == RB_ACT_GELU) {
-    return fmaf(z, kInvSqrt2Pi * expf(-0.5f * z * z), 0.5f * (1.0f + erff(z * kSqrtHalf)));
+    const NormalTail n = normal_tail2(z);
+    const float2 up = __ffma2_rn(n.q, both(-1.0f), both(1.0f));
+    const float2 phi = make_float2(z.x < 0.0f ? n.q.x : up.x, z.y < 0.0f ? n.q.y : up.y);
+    return __ffma2_rn(__fmul2_rn(z, both(kInvSqrt2Pi)), n.e, phi);
   } else if constexpr (kAct == RB_ACT_GELU_TANH) {
-    const float s = sigmoid(kGeluA * fmaf(kGeluB * z * z, z, z));
-    const float t = s * (1.0f - s);  // 0 wherever the polynomial below could overflow
-    return t > 0.0f ? fmaf(z * t, kGeluA * fmaf(3.0f * kGeluB * z, z, 1.0f), s) : s;
-  } else return 1.0f;
+    const float2 s = gelu_tanh_sigmoid2(z);
+    const float2 t = __fmul2_rn(s, __ffma2_rn(s, both(-1.0f), both(1.0f)));
+    const float2 du = __ffma2_rn(__fmul2_rn(z, z), both(3.0f * kGeluA * kGeluB), both(kGeluA));
+    const float2 d = __ffma2_rn(__fmul2_rn(z, t), du, s);
+    return make_float2(t.x > 0.0f ? d.x : s.x, t.y > 0.0f ? d.y : s.y);  // t = 0 wherever du can overflow
+  } else return both(1.0f);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -117,52 +182,53 @@ struct Io;
 
 template <>
 struct Io<__nv_bfloat16> {
-  static __device__ __forceinline__ void load8(float (&v)[8], const __nv_bfloat16* p) {
+  static __device__ __forceinline__ void load8(float2 (&v)[4], const __nv_bfloat16* p) {
     const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = __uint_as_float(w[j] << 16);
-      v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-    }
+    for (int j = 0; j < 4; ++j) v[j] = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
   }
-  static __device__ __forceinline__ void round8(float (&v)[8], uint4& q) {  // v becomes what q holds
-    uint32_t w[4];
+  // Returns the largest magnitude stored, as fp32 bits (NaN above infinity).
+  static __device__ __forceinline__ uint32_t store8(__nv_bfloat16* p, const float2 (&v)[4]) {
+    uint32_t w[4], m = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+      const __nv_bfloat162 b = __float22bfloat162_rn(v[j]);
       w[j] = *reinterpret_cast<const uint32_t*>(&b);
-      v[2 * j] = __uint_as_float(w[j] << 16);
-      v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
     }
-    q = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  static __device__ __forceinline__ void store8(__nv_bfloat16* p, float (&v)[8]) {
-    uint4 q;
-    round8(v, q);
-    *reinterpret_cast<uint4*>(p) = q;
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    return max(m << 16, m & 0xFFFF0000u);
   }
   static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-  static __device__ __forceinline__ float store(__nv_bfloat16* p, float v) {
+  static __device__ __forceinline__ uint32_t store(__nv_bfloat16* p, float v) {
     const __nv_bfloat16 b = __float2bfloat16_rn(v);
     *p = b;
-    return __bfloat162float(b);
+    return __float_as_uint(__bfloat162float(b)) & 0x7FFFFFFFu;
   }
 };
 
 template <>
 struct Io<float> {
-  static __device__ __forceinline__ void load8(float (&v)[8], const float* p) {
+  static __device__ __forceinline__ void load8(float2 (&v)[4], const float* p) {
     const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w);
+    v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
   }
-  static __device__ __forceinline__ void store8(float* p, float (&v)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  static __device__ __forceinline__ uint32_t store8(float* p, const float2 (&v)[4]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      m = max(m, max(__float_as_uint(v[j].x) & 0x7FFFFFFFu, __float_as_uint(v[j].y) & 0x7FFFFFFFu));
+    return m;
   }
   static __device__ __forceinline__ float load(const float* p) { return *p; }
-  static __device__ __forceinline__ float store(float* p, float v) { return *p = v; }
+  static __device__ __forceinline__ uint32_t store(float* p, float v) {
+    *p = v;
+    return __float_as_uint(v) & 0x7FFFFFFFu;
+  }
 };
 
 }  // namespace rb
@@ -172,9 +238,10 @@ namespace rb_host {
 // Device arguments of dropout with probability p (0 <= p <= 1, checked by the caller) and a device seed.
 inline rb::DropoutArgs dropout_args(double p, const int64_t* seed) {
   rb::DropoutArgs d;
-  d.threshold = static_cast<uint32_t>(p * 65536.0 + 0.5);
-  d.scale = d.threshold < 65536u ? static_cast<float>(65536.0 / (65536.0 - d.threshold)) : 0.0f;
-  d.seed = p > 0.0 ? seed : nullptr;
+  const uint32_t threshold = static_cast<uint32_t>(p * 65536.0 + 0.5);
+  d.below = (threshold << 16) - 1u;  // 65536 (everything dropped): above every draw
+  d.scale = threshold < 65536u ? static_cast<float>(65536.0 / (65536.0 - threshold)) : 0.0f;
+  d.seed = threshold > 0 ? seed : nullptr;
   return d;
 }
 
