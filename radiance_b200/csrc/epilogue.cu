@@ -12,33 +12,44 @@ namespace rb {
 // ---------------------------------------------------------------------------------------------
 // Dropout: y = residual + drop(x), flat over n elements
 // ---------------------------------------------------------------------------------------------
-// One group of eight elements (one generator call) per thread and step.  kVec: every pointer is
-// 16-byte aligned; otherwise, and for the last n % 8 elements, elements go one by one.
+// kVec: every pointer is 16-byte aligned.  A thread takes kUnroll groups of eight elements (one generator
+// call each) a step apart and loads them all before it computes: with one group at a time the kernel
+// waited on loads half of the time, at 4.0 TB/s.  Otherwise, and for the last n % 8 elements, elements go
+// one by one.
+constexpr int kUnroll = 2;
+
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* x, const T* residual, T* y, int64_t n,
                                                       const DropoutArgs d) {
   const PhiloxKeys key = philox_keys<true>(d.seed);
-  const int64_t groups = (n + 7) / 8, step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t g = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; g < groups; g += step) {
-    const int64_t i = 8 * g;
-    float2 v[4];
-    if (kVec && i + 8 <= n) {
-      float2 r[4];
-      Io<T>::load8(v, x + i);
-      if (residual != nullptr) Io<T>::load8(r, residual + i);
-      if (d.seed != nullptr) dropout8(v, (uint64_t)g, key, d.below, d.scale);
-      if (residual != nullptr) {
+  const int64_t step = (int64_t)gridDim.x * blockDim.x, first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t groups = kVec ? n / 8 : 0;
+  for (int64_t g0 = first; g0 < groups; g0 += kUnroll * step) {
+    float2 v[kUnroll][4], r[kUnroll][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = __fadd2_rn(v[j], r[j]);
-      }
-      Io<T>::store8(y + i, v);
-    } else {
-      for (int j = 0; j < 8 && i + j < n; ++j) {
-        float u = Io<T>::load(x + i + j);
-        if (d.seed != nullptr) u = dropout1(u, (uint64_t)(i + j), key, d.below, d.scale);
-        Io<T>::store(y + i + j, residual != nullptr ? u + Io<T>::load(residual + i + j) : u);
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t g = g0 + u * step;
+      if (g < groups) {
+        Io<T>::load8(v[u], x + 8 * g);
+        if (residual != nullptr) Io<T>::load8(r[u], residual + 8 * g);
       }
     }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t g = g0 + u * step;
+      if (g >= groups) break;
+      if (d.seed != nullptr) dropout8(v[u], (uint64_t)g, key, d.below, d.scale);
+      if (residual != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[u][j] = __fadd2_rn(v[u][j], r[u][j]);
+      }
+      Io<T>::store8(y + 8 * g, v[u]);
+    }
+  }
+  for (int64_t i = 8 * groups + first; i < n; i += step) {
+    float u = Io<T>::load(x + i);
+    if (d.seed != nullptr) u = dropout1(u, (uint64_t)i, key, d.below, d.scale);
+    Io<T>::store(y + i, residual != nullptr ? u + Io<T>::load(residual + i) : u);
   }
 }
 

@@ -214,11 +214,15 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
 }
 // The output is written once and not read again by this kernel, so its lines are marked to leave
 // L2 first: the operand tiles that later tiles re-read stay resident.
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t smem_src, int x, int y) {
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t smem_src, int x, int y,
+                                             uint64_t policy) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group.L2::cache_hint [%0, {%2, %3}], [%1], %4;" ::"l"(
                    map),
-               "r"(smem_src), "r"(x), "r"(y), "l"(policy_evict_first())
+               "r"(smem_src), "r"(x), "r"(y), "l"(policy)
                : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t smem_src, int x, int y) {
+  tma_store_2d(map, smem_src, x, y, policy_evict_first());
 }
 __device__ __forceinline__ void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // Waits until at most N committed bulk groups of this thread still read their shared-memory source.
@@ -748,7 +752,8 @@ constexpr int kSfStep = 2048;  // one K step's scale atoms for 128 rows (4 x 512
 // What the epilogue does besides alpha, bias and the cast.
 constexpr int kPlain = 0;
 constexpr int kSwigluMode = 1;  // also h = silu(g) * u and its maximum (rb_nvfp4_gemm_swiglu)
-constexpr int kFused = 2;       // activation, dropout, residual (rb_nvfp4_gemm_epilogue)
+constexpr int kFused = 2;       // activation, dropout, residual (rb_nvfp4_gemm_epilogue), bf16 output
+constexpr int kFusedF32 = 3;    // the same with fp32 output
 
 // Per instantiation: the plain GEMM keeps five operand stages and four epilogue warps.  The SwiGLU
 // GEMM's epilogue also computes and stores h, so it runs two epilogue warps on each TMEM lane
@@ -760,6 +765,7 @@ constexpr int kFused = 2;       // activation, dropout, residual (rb_nvfp4_gemm_
 template <int kMode>
 struct Gemm2Cfg {
   static constexpr int kStages = kMode != kPlain ? 4 : 5;
+  static constexpr bool kIsFused = kMode == kFused || kMode == kFusedF32;
   static constexpr int kEpiWarps = kMode != kPlain ? 8 : 4;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;  // producer, MMA issuer, epilogue
   static constexpr int kSwBoxes = 1;                    // SwiGLU mode: staged (output, h) box pairs per warp
@@ -785,13 +791,14 @@ struct Gemm2Smem {
   uint64_t acc_full;                // each CTA: the accumulator of a tile is complete
   uint64_t acc_empty;               // leader: the pair's epilogue warps are done with the shared columns
   uint64_t drain;
-  uint64_t res_full[kMode == kFused ? Gemm2Cfg<kMode>::kOutBoxes : 1];  // fused: a residual box has landed
+  uint64_t res_full[Gemm2Cfg<kMode>::kIsFused ? Gemm2Cfg<kMode>::kOutBoxes : 1];  // fused: a residual has landed
+  float bias[Gemm2Cfg<kMode>::kIsFused ? Gemm2Cfg<kMode>::kEpiWarps : 1][kEpiChunk];  // fused: a chunk's, per warp
   uint32_t tmem_base;
 };
 
 // Dynamic shared memory is the struct plus 1 KB for the 1024-byte alignment; 227 KB per CTA at most.
 static_assert(sizeof(Gemm2Smem<kPlain>) + 1024 <= 232448 && sizeof(Gemm2Smem<kSwigluMode>) + 1024 <= 232448 &&
-                  sizeof(Gemm2Smem<kFused>) + 1024 <= 232448,
+                  sizeof(Gemm2Smem<kFused>) + 1024 <= 232448 && sizeof(Gemm2Smem<kFusedF32>) + 1024 <= 232448,
               "two-SM GEMM shared memory exceeds 227 KB");
 
 constexpr uint32_t kStageBytes2 = 2 * kBM * kStepBytes + 3 * kSfStep;  // per CTA
@@ -931,9 +938,11 @@ __device__ __forceinline__ uint32_t box_chunk(uint32_t row_addr, int c, uint32_t
   return row_addr + (((uint32_t)c ^ sw) << 4);
 }
 
-// Eight values as one (bf16) or two (fp32) chunks, numbered by the eight-column group j of the box.
-__device__ __forceinline__ void box_store8(const float2* v, uint32_t row_addr, int j, uint32_t sw, bool f32) {
-  if (f32) {
+// Eight values to the chunks (one of bf16, two of fp32) of the box's eight-column group j, and the reverse
+// (added).
+template <bool kF32>
+__device__ __forceinline__ void box_store8(const float2* v, uint32_t row_addr, int j, uint32_t sw) {
+  if constexpr (kF32) {
     st_shared_v4(box_chunk(row_addr, 2 * j, sw), __float_as_uint(v[0].x), __float_as_uint(v[0].y),
                  __float_as_uint(v[1].x), __float_as_uint(v[1].y));
     st_shared_v4(box_chunk(row_addr, 2 * j + 1, sw), __float_as_uint(v[2].x), __float_as_uint(v[2].y),
@@ -943,8 +952,9 @@ __device__ __forceinline__ void box_store8(const float2* v, uint32_t row_addr, i
                  pack_bf16x2(v[2].x, v[2].y), pack_bf16x2(v[3].x, v[3].y));
   }
 }
-__device__ __forceinline__ void box_add8(float2* v, uint32_t row_addr, int j, uint32_t sw, bool f32) {
-  if (f32) {
+template <bool kF32>
+__device__ __forceinline__ void box_add8(float2* v, uint32_t row_addr, int j, uint32_t sw) {
+  if constexpr (kF32) {
     const uint4 a = ld_shared_v4(box_chunk(row_addr, 2 * j, sw)), b = ld_shared_v4(box_chunk(row_addr, 2 * j + 1, sw));
     v[0] = __fadd2_rn(v[0], make_float2(__uint_as_float(a.x), __uint_as_float(a.y)));
     v[1] = __fadd2_rn(v[1], make_float2(__uint_as_float(a.z), __uint_as_float(a.w)));
@@ -966,40 +976,29 @@ __device__ __forceinline__ void act32(float2 (&v)[16]) {
 }
 
 // 32 accumulator columns of this lane's row (r), columns col0 .. col0 + 31 of the output, at the box's
-// eight-column groups j0 .. j0 + 3.  Each step runs over all 32 before the next begins, so that its
-// branch is taken once and its latencies overlap (going through all steps eight columns at a time took
-// 1.6 times as long without an activation).  The residual lies in the box where the result goes: each
-// lane replaces its own chunks and needs no one else's.
+// eight-column groups j0 .. j0 + 3; `bias` (shared memory) holds theirs.  Each step runs over all 32 before the
+// next begins, so that its branch is taken once and its latencies overlap (going through all steps eight
+// columns at a time took 1.6 times as long without an activation).  The residual lies in the box where the
+// result goes: each lane replaces its own chunks and needs no one else's.
+template <bool kF32>
 __device__ __forceinline__ void fused_columns(const uint32_t* r, float alpha, const GemmArgs& g, int64_t row, int col0,
-                                              const PhiloxKeys& key, uint32_t row_addr, uint32_t zrow_addr, int j0,
-                                              uint32_t sw) {
-  const bool f32 = g.out_f32 != 0;
+                                              const PhiloxKeys& key, const float* bias, uint32_t row_addr,
+                                              uint32_t zrow_addr, int j0, uint32_t sw) {
   float2 v[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     v[i] = __fmul2_rn(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), both(alpha));
   if (g.bias != nullptr) {
-    if (g.bias_f32) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float2 b[4];
-        Io<float>::load8(b, reinterpret_cast<const float*>(g.bias) + col0 + 8 * j);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * j + i] = __fadd2_rn(v[4 * j + i], b[i]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float2 b[4];
-        Io<__nv_bfloat16>::load8(b, reinterpret_cast<const __nv_bfloat16*>(g.bias) + col0 + 8 * j);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * j + i] = __fadd2_rn(v[4 * j + i], b[i]);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const float4 b = reinterpret_cast<const float4*>(bias)[i];
+      v[2 * i] = __fadd2_rn(v[2 * i], make_float2(b.x, b.y));
+      v[2 * i + 1] = __fadd2_rn(v[2 * i + 1], make_float2(b.z, b.w));
     }
   }
   if (g.has_preact) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) box_store8(v + 4 * j, zrow_addr, j0 + j, sw, f32);
+    for (int j = 0; j < 4; ++j) box_store8<kF32>(v + 4 * j, zrow_addr, j0 + j, sw);
   }
   switch (g.act) {
     case RB_ACT_RELU: act32<RB_ACT_RELU>(v); break;
@@ -1017,53 +1016,78 @@ __device__ __forceinline__ void fused_columns(const uint32_t* r, float alpha, co
   }
   if (g.has_residual) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) box_add8(v + 4 * j, row_addr, j0 + j, sw, f32);
+    for (int j = 0; j < 4; ++j) box_add8<kF32>(v + 4 * j, row_addr, j0 + j, sw);
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) box_store8(v + 4 * j, row_addr, j0 + j, sw, f32);
+  for (int j = 0; j < 4; ++j) box_store8<kF32>(v + 4 * j, row_addr, j0 + j, sw);
 }
 
-// One epilogue warp of the two-SM kernel in fused mode.  Its work is a sequence of pieces, one box (32
-// rows x 128 bytes: 64 bf16 or 32 fp32 columns) each.  The residual of a piece is loaded by TMA into the
-// box that the piece is staged in, replaced there element by element and stored by TMA.  The warp's two
-// boxes alternate, and while one piece is computed the next one's residual (the next tile's, after the
-// last) is on its way; with the pre-activations kept, the second box holds them and the residual is
-// loaded when its piece begins.
-template <class Smem>
+// One epilogue warp of the two-SM kernel in fused mode: the TMEM lanes of its warp id mod 4, and every other
+// 64-column chunk of the tile.  It stages its results in boxes of 32 rows x 128 bytes: a chunk is one box of
+// bf16 or two of fp32.  The residual of a box is loaded by TMA into the box that its result is staged in,
+// replaced there element by element and stored by TMA.  The warp has two boxes, and what fits them both
+// shares one wait for earlier stores and has its residuals loaded together: a tile's two chunks (bf16),
+// before the wait for the accumulator, or a chunk (fp32).  With the pre-activations kept, the second box
+// holds them, and every box has a wait of its own.
+// The bias of the next chunk is on its way while a chunk is computed: loaded when it is needed, it missed
+// L1 on every tile's new columns and took 1800 of an epilogue's 8400 cycles a tile (no activation).
+template <bool kF32, class Smem>
 __device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, const CUtensorMap& tmO,
                                                const CUtensorMap& tmZ, const CUtensorMap& tmR, int cid, int ncl,
                                                int n_my, uint32_t rank, int warp, int lane) {
+  constexpr int kParts = kF32 ? 2 : 1, kBoxCols = kEpiChunk / kParts;
   const int q = warp & 3, ew = warp - 2, half = ew / 4;
   const uint32_t boxes = smem_u32(&sm.out[2 * ew][0]);
   uint64_t* bars = &sm.res_full[2 * ew];
-  const bool f32 = g.out_f32 != 0, residual = g.has_residual != 0, preact = g.has_preact != 0;
-  const bool ahead = residual && !preact;  // residuals are loaded one piece ahead
-  const int parts = f32 ? 2 : 1;           // pieces of a 64-column chunk
+  float* bias_sm = sm.bias[ew];
+  const bool residual = g.has_residual != 0, preact = g.has_preact != 0;
   const PhiloxKeys key = philox_keys<false>(g.drop.seed);
   const uint32_t sw = (uint32_t)(lane & 7), lane_row = (uint32_t)lane * 128u;
+  const uint64_t policy = policy_evict_first();
+  float alpha = 1.0f;
+  if (g.alpha_a != nullptr) alpha = __ldg(g.alpha_a);
+  if (g.alpha_b != nullptr) alpha = __fmul_rn(alpha, __ldg(g.alpha_b));
   const auto row_of = [&](const Tile2& T) { return T.orow + (int64_t)rank * kBM + 32 * q; };
   // The 64-column chunk that tile i's shared columns [192, 256) hold, or -1 (see the plain epilogue).
   const auto shared_chunk = [&](int i, int width) { return (i & 1) ? 0 : (width == kBN ? width / kEpiChunk - 1 : -1); };
-  // This warp's chunk at `step` of tile i: ascending, except that buffer 0's shared last chunk goes first.
-  const auto chunk_at = [&](int i, int width, int step) {
+  // First column in tile i of this warp's chunk at `step`: ascending, except that buffer 0's shared last chunk
+  // goes first.
+  const auto column_at = [&](int i, int width, int step) {
     const int sc = shared_chunk(i, width);
     const bool first = sc >= 0 && (sc & 1) == half && !(i & 1);
-    return first ? (step == 0 ? sc : half + (step - 1) * 2) : half + step * 2;
+    return (first ? (step == 0 ? sc : half + (step - 1) * 2) : half + step * 2) * kEpiChunk;
+  };
+  // This lane's two columns of a chunk's bias.
+  const auto load_bias = [&](int col) {
+    if (g.bias == nullptr) return both(0.0f);
+    if (g.bias_f32) return __ldg(reinterpret_cast<const float2*>(reinterpret_cast<const float*>(g.bias) + col) + lane);
+    const uint32_t w = __ldg(reinterpret_cast<const unsigned int*>(reinterpret_cast<const uint16_t*>(g.bias) + col) + lane);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
   };
   const auto load_residual = [&](int slot, int64_t row, int col) {
     mbar_arrive_expect_tx(&bars[slot], kOutBox);
     tma_load_2d(reinterpret_cast<void*>(&sm.out[2 * ew + slot][0]), &tmR, &bars[slot], col, (int)row);
   };
   Tile2 T = tile2_at(cid, g, sm.tile_prefix);
+  float2 next_bias = n_my > 0 ? load_bias(T.ncol0 + column_at(0, T.width, 0)) : both(0.0f);
   uint32_t phases = 0;  // bit s: the parity that box s's next residual completes
-  int slot = 0;
-  if (ahead && n_my > 0 && lane == 0 && row_of(T) < T.row_end)
-    load_residual(0, row_of(T), T.ncol0 + chunk_at(0, T.width, 0) * kEpiChunk);
   for (int i = 0; i < n_my; ++i) {
-    const Tile2 Tn = i + 1 < n_my ? tile2_at(cid + (i + 1) * ncl, g, sm.tile_prefix) : T;
-    float alpha = 1.0f;
-    if (g.alpha_a != nullptr) alpha = __ldg(g.alpha_a);
-    if (g.alpha_b != nullptr) alpha = __fmul_rn(alpha, __ldg(g.alpha_b));
+    const int64_t row0 = row_of(T);
+    const bool store = row0 < T.row_end;
+    const int steps = T.width / (2 * kEpiChunk);  // this warp's chunks
+    // Frees the boxes and loads the residuals that go into them: of the chunk at `step`, part `part` (and with
+    // both boxes for results, of the part or step after it).
+    const auto open_boxes = [&](int step, int part) {
+      if (lane != 0) return;
+      bulk_wait_read<0>();
+      if (!residual || !store) return;
+      const int col = T.ncol0 + column_at(i, T.width, step);
+      load_residual(0, row0, col + part * kBoxCols);
+      if (preact) return;
+      if constexpr (kF32) load_residual(1, row0, col + kBoxCols);
+      else if (step + 1 < steps) load_residual(1, row0, T.ncol0 + column_at(i, T.width, step + 1));
+    };
+    open_boxes(0, 0);
     if (!__all_sync(0xFFFFFFFFu, mbar_wait_sleep(&sm.acc_full, (uint32_t)(i & 1), 64))) {
       if (lane == 0) record_status(&g_gemm_status, kStatusTimeoutMma);
       return;
@@ -1077,42 +1101,31 @@ __device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, cons
       else mbar_arrive_leader(&sm.acc_empty);
     };
     if (!mine_sc && lane == 0) release();
-    const int64_t row0 = row_of(T);
-    const bool store = row0 < T.row_end;
-    const int nmine = T.width / (2 * kEpiChunk);
-    for (int step = 0; step < nmine; ++step) {
-      const int c = chunk_at(i, T.width, step);
+    for (int step = 0; step < steps; ++step) {
+      const int col = column_at(i, T.width, step);
       uint32_t r[kEpiChunk];
-      const uint32_t taddr = ((uint32_t)(32 * q) << 16) + (uint32_t)(base_col + c * kEpiChunk);
+      const uint32_t taddr = ((uint32_t)(32 * q) << 16) + (uint32_t)(base_col + col);
       RB_TMEM_LD_X32(taddr, r);
       RB_TMEM_LD_X32(taddr + 32, (r + 32));
+      if (g.bias != nullptr) reinterpret_cast<float2*>(bias_sm)[lane] = next_bias;
+      if (step > 0 && (kF32 || preact)) open_boxes(step, 0);
       tmem_ld_wait();
-      if (step == 0 && mine_sc) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) release();
+      if (step == 0 && mine_sc) tc_fence_before();
+      __syncwarp();
+      if (step == 0 && mine_sc && lane == 0) release();
+      if (step + 1 < steps) {
+        next_bias = load_bias(T.ncol0 + column_at(i, T.width, step + 1));
+      } else if (i + 1 < n_my) {
+        const Tile2 Tn = tile2_at(cid + (i + 1) * ncl, g, sm.tile_prefix);
+        next_bias = load_bias(Tn.ncol0 + column_at(i + 1, Tn.width, 0));
       }
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        if (part >= parts) break;
-        const int col0 = T.ncol0 + c * kEpiChunk + 32 * part;
-        if (lane == 0) {
-          // The box to write into (or to load the next residual into) is read by no store any more.
-          if (residual || preact) bulk_wait_read<0>();
-          else bulk_wait_read<1>();
-          if (ahead) {
-            if (part + 1 < parts) {
-              if (store) load_residual(slot ^ 1, row0, col0 + 32);
-            } else if (step + 1 < nmine) {
-              if (store) load_residual(slot ^ 1, row0, T.ncol0 + chunk_at(i, T.width, step + 1) * kEpiChunk);
-            } else if (i + 1 < n_my && row_of(Tn) < Tn.row_end) {
-              load_residual(slot ^ 1, row_of(Tn), Tn.ncol0 + chunk_at(i + 1, Tn.width, 0) * kEpiChunk);
-            }
-          } else if (residual && store) {
-            load_residual(0, row0, col0);
-          }
+      for (int part = 0; part < kParts; ++part) {
+        if (part > 0 && preact) {
+          open_boxes(step, part);
+          __syncwarp();
         }
-        __syncwarp();
+        const int slot = preact ? 0 : kF32 ? part : step;
         if (residual && store) {
           if (!mbar_wait_warp(&bars[slot], (phases >> slot) & 1u)) {
             if (lane == 0) record_status(&g_gemm_status, kStatusTimeoutTma);
@@ -1120,24 +1133,27 @@ __device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, cons
           }
           phases ^= 1u << slot;
         }
-        const uint32_t row_addr = boxes + (uint32_t)slot * kOutBox + lane_row, zrow_addr = boxes + kOutBox + lane_row;
-        if (f32) {
-          fused_columns(r + 32 * part, alpha, g, row0 + lane, col0, key, row_addr, zrow_addr, 0, sw);
+        const int box_col = T.ncol0 + col + part * kBoxCols;
+        const uint32_t box = boxes + (uint32_t)slot * kOutBox;
+        const uint32_t row_addr = box + lane_row, zrow_addr = boxes + kOutBox + lane_row;
+        if constexpr (kF32) {
+          fused_columns<true>(r + 32 * part, alpha, g, row0 + lane, box_col, key, bias_sm + 32 * part, row_addr,
+                              zrow_addr, 0, sw);
         } else {
-          fused_columns(r, alpha, g, row0 + lane, col0, key, row_addr, zrow_addr, 0, sw);
-          fused_columns(r + 32, alpha, g, row0 + lane, col0 + 32, key, row_addr, zrow_addr, 4, sw);
+          fused_columns<false>(r, alpha, g, row0 + lane, box_col, key, bias_sm, row_addr, zrow_addr, 0, sw);
+          fused_columns<false>(r + 32, alpha, g, row0 + lane, box_col + 32, key, bias_sm + 32, row_addr, zrow_addr, 4,
+                               sw);
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0 && store) {
-          tma_store_2d(&tmO, boxes + (uint32_t)slot * kOutBox, col0, (int)row0);
-          if (preact) tma_store_2d(&tmZ, boxes + kOutBox, col0, (int)row0);
+          tma_store_2d(&tmO, box, box_col, (int)row0, policy);
+          if (preact) tma_store_2d(&tmZ, boxes + kOutBox, box_col, (int)row0, policy);
           bulk_commit_group();
         }
-        if (!preact) slot ^= 1;
       }
     }
-    T = Tn;
+    T = tile2_at(min(cid + (i + 1) * ncl, g.n_tiles - 1), g, sm.tile_prefix);
   }
 }
 
@@ -1190,7 +1206,7 @@ __global__ void __launch_bounds__(Gemm2Cfg<kMode>::kThreads, 1)
     mbar_init(&sm.acc_full, 1);
     mbar_init(&sm.acc_empty, 2 * kEW);
     mbar_init(&sm.drain, 1);
-    if constexpr (kMode == kFused)
+    if constexpr (Gemm2Cfg<kMode>::kIsFused)
       for (int b = 0; b < Gemm2Cfg<kMode>::kOutBoxes; ++b) mbar_init(&sm.res_full[b], 1);
     fence_mbar_init();
     prefetch_tensormap(&tmA);
@@ -1199,7 +1215,7 @@ __global__ void __launch_bounds__(Gemm2Cfg<kMode>::kThreads, 1)
     prefetch_tensormap(&tmSB);
     prefetch_tensormap(&tmO);
     if constexpr (kSwiglu) prefetch_tensormap(&tmH);
-    if constexpr (kMode == kFused) {
+    if constexpr (Gemm2Cfg<kMode>::kIsFused) {
       if (g.has_preact) prefetch_tensormap(&tmH);
       if (g.has_residual) prefetch_tensormap(&tmR);
     }
@@ -1330,8 +1346,8 @@ __global__ void __launch_bounds__(Gemm2Cfg<kMode>::kThreads, 1)
     const int q = warp & 3;  // TMEM lanes 32q .. 32q+31
     constexpr int kStride = kEW / 4;
     const int half = (warp - 2) / 4;
-    if constexpr (kMode == kFused) {
-      fused_epilogue(sm, g, tmO, tmH, tmR, cid, ncl, n_my, rank, warp, lane);
+    if constexpr (Gemm2Cfg<kMode>::kIsFused) {
+      fused_epilogue<kMode == kFusedF32>(sm, g, tmO, tmH, tmR, cid, ncl, n_my, rank, warp, lane);
     } else {
     // Staging: two boxes per warp (pieces alternate between them), or in SwiGLU mode kSwBoxes
     // (output, h) box pairs per warp.
@@ -1696,8 +1712,9 @@ static int gemm_impl(const void* a_packed, const void* a_scale, const void* b_pa
                                                             (uint64_t)fe.ldr * oesize, 128 / oesize, 32,
                                                             CU_TENSOR_MAP_SWIZZLE_128B)))
         return RB_ERR_CUDA;
-      return launch_two_sm<kFused>(g, tmA, tmB, tmO, a_scale, m, b_scale, n, g.n_tiles, dev, st,
-                                   fe.preact != nullptr ? &tmZ : nullptr, fe.residual != nullptr ? &tmR : nullptr);
+      const CUtensorMap *z = fe.preact != nullptr ? &tmZ : nullptr, *r = fe.residual != nullptr ? &tmR : nullptr;
+      return g.out_f32 ? launch_two_sm<kFusedF32>(g, tmA, tmB, tmO, a_scale, m, b_scale, n, g.n_tiles, dev, st, z, r)
+                       : launch_two_sm<kFused>(g, tmA, tmB, tmO, a_scale, m, b_scale, n, g.n_tiles, dev, st, z, r);
     }
     if (swiglu) {
       // h boxes: 32 rows x 32 bf16 (64 bytes), 64-byte swizzled; rows past m are clipped.
