@@ -469,190 +469,302 @@ struct RowsArgs {
   float* grad_w;         // combine backward: tokens x k
   int64_t tokens, d, num_rows;
   int k;
-  int cx;                // threads along a row (a power of two, 32 .. 256)
+  int cx;                // threads to a token (a power of two, 32 .. 256)
   // dispatch and combine backward: the rows that no pair fills become zero
   const int64_t* counts;
   const int64_t* offsets;
   int experts, pad_slices;
-  int64_t token_blocks;
 };
 
-// kVec elements of T as one load (16 bytes, or one element where rows are not 16-byte aligned).
+// kVec elements of T as one load: 16 bytes, or one element where rows are not 16-byte aligned.  get and set
+// turn them into fp32 and back (rounded).
 template <typename T, int kVec>
-struct Pack {
-  T v[kVec];
+struct Pack;
+template <>
+struct Pack<__nv_bfloat16, 8> {
+  uint4 q;
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    q = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <>
+struct Pack<float, 4> {
+  uint4 q;
+  __device__ __forceinline__ void get(float (&f)[4]) const {
+    f[0] = __uint_as_float(q.x), f[1] = __uint_as_float(q.y), f[2] = __uint_as_float(q.z), f[3] = __uint_as_float(q.w);
+  }
+  __device__ __forceinline__ void set(const float (&f)[4]) {
+    q = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <>
+struct Pack<__nv_bfloat16, 1> {
+  __nv_bfloat16 q;
+  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = __bfloat162float(q); }
+  __device__ __forceinline__ void set(const float (&f)[1]) { q = __float2bfloat16_rn(f[0]); }
+};
+template <>
+struct Pack<float, 1> {
+  float q;
+  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = q; }
+  __device__ __forceinline__ void set(const float (&f)[1]) { q = f[0]; }
 };
 template <typename T, int kVec>
 __device__ __forceinline__ Pack<T, kVec> load_pack(const T* p) {
   Pack<T, kVec> r;
-  if constexpr (kVec * sizeof(T) == 16) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-    r = *reinterpret_cast<const Pack<T, kVec>*>(&q);
-  } else {
-    r.v[0] = *p;
-  }
+  if constexpr (kVec > 1) r.q = __ldg(reinterpret_cast<const uint4*>(p));
+  else r.q = *p;
   return r;
 }
 template <typename T, int kVec>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, kVec>& r) {
-  if constexpr (kVec * sizeof(T) == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
-  else *p = r.v[0];
-}
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ void from_f(__nv_bfloat16& o, float v) { o = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void from_f(float& o, float v) { o = v; }
-
-// The row of a pair, or -1 where the pair has none (a row outside the layout is never touched).
-__device__ __forceinline__ int64_t pair_row(const RowsArgs& a, int64_t t, int j) {
-  const int64_t r = __ldg(a.rows + t * a.k + j);
-  return r < a.num_rows ? r : -1;
+  if constexpr (kVec > 1) *reinterpret_cast<uint4*>(p) = r.q;
+  else *p = r.q;
 }
 
-// Zeroes the rows that hold no pair: the end of every expert's group and the rows past the last
-// group.  Each is one run of consecutive rows; `pad_slices` blocks share an expert's, all share the last.
-template <typename T, int kVec>
-__device__ __forceinline__ void zero_unused_rows(const RowsArgs& a, int64_t b) {
-  const int e = (int)(b / a.pad_slices);
-  const int64_t slice = b % a.pad_slices, blocks = (int64_t)a.experts * a.pad_slices;
-  const int cx = a.cx, ty = (int)threadIdx.x / cx, ny = 256 / cx, x = (int)threadIdx.x % cx;
-  T* out = reinterpret_cast<T*>(a.out);
-  Pack<T, kVec> zero;
+// Up to kP pairs of a token: their rows (-1 without one; a row outside the layout is never touched) and weights.
+template <int kP>
+struct Pairs {
+  int32_t row[kP];
+  float w[kP];
+};
+template <int kP>
+__device__ __forceinline__ Pairs<kP> load_pairs(const RowsArgs& a, int64_t t, int j0) {
+  Pairs<kP> p;
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) from_f(zero.v[i], 0.0f);
+  for (int u = 0; u < kP; ++u) {
+    const bool in = t < a.tokens && j0 + u < a.k;
+    const int32_t r = in ? __ldg(a.rows + t * a.k + j0 + u) : -1;
+    p.row[u] = r < a.num_rows ? r : -1;
+    p.w[u] = in && a.weights != nullptr ? __ldg(a.weights + t * a.k + j0 + u) : 1.0f;
+  }
+  return p;
+}
+
+// Zeroes the rows that hold no pair: the end of every expert's group and the rows past the last group.  Each
+// is one run of consecutive rows.  A group's run is cut into `pad_slices` pieces, and the pieces of all
+// groups are dealt to the blocks; the last run is dealt to all blocks row by row.
+template <typename T, int kVec>
+__device__ __forceinline__ void zero_unused_rows(const RowsArgs& a) {
+  const int ty = (int)threadIdx.x / a.cx, ny = 256 / a.cx, x = (int)threadIdx.x % a.cx;
+  T* out = reinterpret_cast<T*>(a.out);
+  const float none[kVec] = {};
+  Pack<T, kVec> zero;
+  zero.set(none);
   const auto clear = [&](int64_t r0, int64_t r1, int64_t first, int64_t step) {
     r0 = max(r0, (int64_t)0);
     r1 = min(r1, a.num_rows);
     for (int64_t r = r0 + first; r < r1; r += step)
-      for (int64_t c = (int64_t)x * kVec; c < a.d; c += (int64_t)cx * kVec) store_pack<T, kVec>(out + r * a.ld_out + c, zero);
+      for (int64_t c = (int64_t)x * kVec; c < a.d; c += (int64_t)a.cx * kVec)
+        store_pack<T, kVec>(out + r * a.ld_out + c, zero);
   };
-  clear(a.offsets[e] + a.counts[e], a.offsets[e + 1], slice * ny + ty, (int64_t)a.pad_slices * ny);
-  clear(a.offsets[a.experts], a.num_rows, b * ny + ty, blocks * ny);
+  for (int b = blockIdx.x; b < a.experts * a.pad_slices; b += gridDim.x) {
+    const int e = b / a.pad_slices, slice = b % a.pad_slices;
+    clear(a.offsets[e] + a.counts[e], a.offsets[e + 1], (int64_t)slice * ny + ty, (int64_t)a.pad_slices * ny);
+  }
+  clear(a.offsets[a.experts], a.num_rows, (int64_t)blockIdx.x * ny + ty, (int64_t)gridDim.x * ny);
 }
 
-// x[t] to the row of each of its pairs.  A token's row is read once and written k times; cx threads
-// cover it, 256 / cx tokens to a block.
-template <typename T, int kVec>
-__global__ void __launch_bounds__(256) token_dispatch_kernel(const RowsArgs a) {
-  if ((int64_t)blockIdx.x >= a.token_blocks) {
-    zero_unused_rows<T, kVec>(a, (int64_t)blockIdx.x - a.token_blocks);
-    return;
-  }
-  const int cx = a.cx, x = (int)threadIdx.x % cx;
-  const int64_t t = (int64_t)blockIdx.x * (256 / cx) + (int)threadIdx.x / cx;
-  if (t >= a.tokens) return;
-  const T* src = reinterpret_cast<const T*>(a.src) + t * a.ld_src;
+// The three moves below share a shape: cx threads take a token (a warp when there are tokens for every
+// resident warp, more for a few tokens), every thread kCols vectors of its row and kP of its pairs at a time, and
+// the tokens are dealt to as many blocks as are resident.  A token's rows and weights are loaded while the
+// token before it is moved, and a warp reads long pieces of a row (2 KB) with many loads in flight, two
+// blocks to an SM: 16384 tokens x 2048, k = 2 with a residual, combine in 47 us (268 MB, 5.7 TB/s).  One
+// vector a thread at higher occupancy, each token waiting for its rows and only then for its data: 96 us;
+// four vectors but three blocks, with registers spilled: 75 us.
+constexpr int kRowsBlocksPerSm = 2;
+constexpr int kRowsCols2 = 4;  // vectors at a time for up to two pairs
+constexpr int kRowsCols4 = 2;  // and for four pairs at a time
+
+// x[t] to the row of each of its pairs: a token's row is read once and written k times.
+template <typename T, int kVec, int kP, int kCols>
+__global__ void __launch_bounds__(256, kRowsBlocksPerSm) token_dispatch_kernel(const RowsArgs a) {
+  zero_unused_rows<T, kVec>(a);
+  const int cx = a.cx, ny = 256 / cx, x = (int)threadIdx.x % cx;
+  const int64_t step = (int64_t)gridDim.x * ny, wide = (int64_t)cx * kVec;
   T* out = reinterpret_cast<T*>(a.out);
-  for (int64_t c = (int64_t)x * kVec; c < a.d; c += (int64_t)cx * kVec) {
-    const Pack<T, kVec> v = load_pack<T, kVec>(src + c);
-    for (int j = 0; j < a.k; ++j) {
-      const int64_t r = pair_row(a, t, j);
-      if (r >= 0) store_pack<T, kVec>(out + r * a.ld_out + c, v);
+  int64_t t = (int64_t)blockIdx.x * ny + (int)threadIdx.x / cx;
+  Pairs<kP> next = load_pairs<kP>(a, t, 0);
+  for (; t < a.tokens; t += step) {
+    const Pairs<kP> first = next;
+    next = load_pairs<kP>(a, t + step, 0);
+    const T* src = reinterpret_cast<const T*>(a.src) + t * a.ld_src;
+    for (int64_t c = (int64_t)x * kVec; c < a.d; c += kCols * wide) {
+      Pack<T, kVec> v[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i)
+        if (c + i * wide < a.d) v[i] = load_pack<T, kVec>(src + c + i * wide);
+      for (int j0 = 0; j0 < a.k; j0 += kP) {
+        const Pairs<kP> p = j0 == 0 ? first : load_pairs<kP>(a, t, j0);
+#pragma unroll
+        for (int u = 0; u < kP; ++u)
+          if (p.row[u] >= 0) {
+#pragma unroll
+            for (int i = 0; i < kCols; ++i)
+              if (c + i * wide < a.d) store_pack<T, kVec>(out + p.row[u] * a.ld_out + c + i * wide, v[i]);
+          }
+      }
     }
   }
 }
 
 // y[t] = residual[t] + sum_j w[t, j] rows[row(t, j)], in fp32 and in the order of j, rounded once.
-// Without weights it is the dispatch's backward.  Four rows are loaded at a time.
-template <typename T, int kVec>
-__global__ void __launch_bounds__(256) token_combine_kernel(const RowsArgs a) {
-  const int cx = a.cx, x = (int)threadIdx.x % cx;
-  const int64_t t = (int64_t)blockIdx.x * (256 / cx) + (int)threadIdx.x / cx;
-  if (t >= a.tokens) return;
+// Without weights it is the dispatch's backward.
+template <typename T, int kVec, int kP, int kCols>
+__global__ void __launch_bounds__(256, kRowsBlocksPerSm) token_combine_kernel(const RowsArgs a) {
+  const int cx = a.cx, ny = 256 / cx, x = (int)threadIdx.x % cx;
+  const int64_t step = (int64_t)gridDim.x * ny, wide = (int64_t)cx * kVec;
   const T* src = reinterpret_cast<const T*>(a.src);
-  const T* res = a.extra != nullptr ? reinterpret_cast<const T*>(a.extra) + t * a.ld_extra : nullptr;
-  T* out = reinterpret_cast<T*>(a.out) + t * a.ld_out;
-  for (int64_t c = (int64_t)x * kVec; c < a.d; c += (int64_t)cx * kVec) {
-    float acc[kVec];
+  int64_t t = (int64_t)blockIdx.x * ny + (int)threadIdx.x / cx;
+  Pairs<kP> next = load_pairs<kP>(a, t, 0);
+  for (; t < a.tokens; t += step) {
+    const Pairs<kP> first = next;
+    next = load_pairs<kP>(a, t + step, 0);
+    const T* res = a.extra != nullptr ? reinterpret_cast<const T*>(a.extra) + t * a.ld_extra : nullptr;
+    T* out = reinterpret_cast<T*>(a.out) + t * a.ld_out;
+    for (int64_t c = (int64_t)x * kVec; c < a.d; c += kCols * wide) {
+      float acc[kCols][kVec];
+      Pack<T, kVec> rv[kCols];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) acc[i] = 0.0f;
-    Pack<T, kVec> rv;
-    if (res != nullptr) rv = load_pack<T, kVec>(res + c);
-    for (int j0 = 0; j0 < a.k; j0 += 4) {
-      Pack<T, kVec> v[4];
-      int64_t r[4];
+      for (int i = 0; i < kCols; ++i) {
+        if (res != nullptr && c + i * wide < a.d) rv[i] = load_pack<T, kVec>(res + c + i * wide);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        r[u] = j0 + u < a.k ? pair_row(a, t, j0 + u) : -1;
-        if (r[u] >= 0) v[u] = load_pack<T, kVec>(src + r[u] * a.ld_src + c);
+        for (int e = 0; e < kVec; ++e) acc[i][e] = 0.0f;
+      }
+      for (int j0 = 0; j0 < a.k; j0 += kP) {
+        const Pairs<kP> p = j0 == 0 ? first : load_pairs<kP>(a, t, j0);
+        Pack<T, kVec> v[kP][kCols];
+#pragma unroll
+        for (int u = 0; u < kP; ++u)
+#pragma unroll
+          for (int i = 0; i < kCols; ++i)
+            if (p.row[u] >= 0 && c + i * wide < a.d)
+              v[u][i] = load_pack<T, kVec>(src + p.row[u] * a.ld_src + c + i * wide);
+#pragma unroll
+        for (int u = 0; u < kP; ++u) {
+          if (p.row[u] < 0) continue;
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) {
+            float f[kVec];
+            v[u][i].get(f);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) acc[i][e] = fmaf(p.w[u], f[e], acc[i][e]);
+          }
+        }
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (r[u] < 0) continue;
-        const float w = a.weights != nullptr ? __ldg(a.weights + t * a.k + j0 + u) : 1.0f;
+      for (int i = 0; i < kCols; ++i) {
+        if (c + i * wide >= a.d) continue;
+        if (res != nullptr) {
+          float f[kVec];
+          rv[i].get(f);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) acc[i] = fmaf(w, to_f(v[u].v[i]), acc[i]);
+          for (int e = 0; e < kVec; ++e) acc[i][e] += f[e];
+        }
+        Pack<T, kVec> o;
+        o.set(acc[i]);
+        store_pack<T, kVec>(out + c + i * wide, o);
       }
     }
-    if (res != nullptr) {
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) acc[i] += to_f(rv.v[i]);
-    }
-    Pack<T, kVec> o;
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) from_f(o.v[i], acc[i]);
-    store_pack<T, kVec>(out + c, o);
   }
 }
 
 // grad_rows[row(t, j)] = w[t, j] grad_y[t] and grad_w[t, j] = <grad_y[t], rows[row(t, j)]>.  grad_y's
-// row is read once for four pairs; each pair's product is summed over its cx threads in a fixed order.
-template <typename T, int kVec>
-__global__ void __launch_bounds__(256) token_combine_backward_kernel(const RowsArgs a) {
-  if ((int64_t)blockIdx.x >= a.token_blocks) {
-    zero_unused_rows<T, kVec>(a, (int64_t)blockIdx.x - a.token_blocks);
-    return;
-  }
-  __shared__ float red[8][4];
-  const int cx = a.cx, x = (int)threadIdx.x % cx, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * (256 / cx) + (int)threadIdx.x / cx;
-  const bool in_t = t < a.tokens;
+// row is read once for kP pairs; each pair's product is summed over its cx threads in a fixed order.
+template <typename T, int kVec, int kP, int kCols>
+__global__ void __launch_bounds__(256, kRowsBlocksPerSm) token_combine_backward_kernel(const RowsArgs a) {
+  __shared__ float red[2][8][kP];
+  zero_unused_rows<T, kVec>(a);
+  const int cx = a.cx, ny = 256 / cx, x = (int)threadIdx.x % cx, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t step = (int64_t)gridDim.x * ny, wide = (int64_t)cx * kVec;
   const T* src = reinterpret_cast<const T*>(a.src);
-  const T* gy = reinterpret_cast<const T*>(a.extra) + t * a.ld_extra;
   T* out = reinterpret_cast<T*>(a.out);
-  for (int j0 = 0; j0 < a.k; j0 += 4) {
-    int64_t r[4];
-    float w[4], dot[4];
+  int buf = 0;
+  int64_t t = (int64_t)blockIdx.x * ny + (int)threadIdx.x / cx;
+  Pairs<kP> next = load_pairs<kP>(a, t, 0);
+  // Every thread of the block makes the same number of turns: they meet at the barrier below.
+  for (int64_t tb = (int64_t)blockIdx.x * ny; tb < a.tokens; tb += step, t += step) {
+    const Pairs<kP> first = next;
+    next = load_pairs<kP>(a, t + step, 0);
+    const bool in_t = t < a.tokens;
+    const T* gy = reinterpret_cast<const T*>(a.extra) + (in_t ? t : 0) * a.ld_extra;
+    for (int j0 = 0; j0 < a.k; j0 += kP) {
+      const Pairs<kP> p = j0 == 0 ? first : load_pairs<kP>(a, t, j0);
+      float dot[kP] = {};
+      if (in_t) {
+        for (int64_t c = (int64_t)x * kVec; c < a.d; c += kCols * wide) {
+          Pack<T, kVec> g[kCols], v[kP][kCols];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      r[u] = in_t && j0 + u < a.k ? pair_row(a, t, j0 + u) : -1;
-      w[u] = r[u] >= 0 ? __ldg(a.weights + t * a.k + j0 + u) : 0.0f;
-      dot[u] = 0.0f;
-    }
-    if (in_t) {
-      for (int64_t c = (int64_t)x * kVec; c < a.d; c += (int64_t)cx * kVec) {
-        const Pack<T, kVec> g = load_pack<T, kVec>(gy + c);
-        Pack<T, kVec> v[4];
+          for (int i = 0; i < kCols; ++i) {
+            if (c + i * wide >= a.d) continue;
+            g[i] = load_pack<T, kVec>(gy + c + i * wide);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (r[u] >= 0) v[u] = load_pack<T, kVec>(src + r[u] * a.ld_src + c);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (r[u] < 0) continue;
-          Pack<T, kVec> o;
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            const float gf = to_f(g.v[i]);
-            dot[u] = fmaf(gf, to_f(v[u].v[i]), dot[u]);
-            from_f(o.v[i], w[u] * gf);
+            for (int u = 0; u < kP; ++u)
+              if (p.row[u] >= 0) v[u][i] = load_pack<T, kVec>(src + p.row[u] * a.ld_src + c + i * wide);
           }
-          store_pack<T, kVec>(out + r[u] * a.ld_out + c, o);
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) {
+            if (c + i * wide >= a.d) continue;
+            float gf[kVec];
+            g[i].get(gf);
+#pragma unroll
+            for (int u = 0; u < kP; ++u) {
+              if (p.row[u] < 0) continue;
+              float f[kVec];
+              v[u][i].get(f);
+#pragma unroll
+              for (int e = 0; e < kVec; ++e) {
+                dot[u] = fmaf(gf[e], f[e], dot[u]);
+                f[e] = p.w[u] * gf[e];
+              }
+              Pack<T, kVec> o;
+              o.set(f);
+              store_pack<T, kVec>(out + p.row[u] * a.ld_out + c + i * wide, o);
+            }
+          }
         }
       }
-    }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kP; ++u) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) dot[u] += __shfl_xor_sync(0xFFFFFFFFu, dot[u], o);
-      if (lane == 0) red[warp][u] = dot[u];
+        for (int o = 16; o > 0; o >>= 1) dot[u] += __shfl_xor_sync(0xFFFFFFFFu, dot[u], o);
+      }
+      if (cx == 32) {  // a warp to a token
+        float s = dot[0];
+#pragma unroll
+        for (int u = 1; u < kP; ++u)
+          if (lane == u) s = dot[u];
+        if (in_t && lane < kP && j0 + lane < a.k) a.grad_w[t * a.k + j0 + lane] = s;
+        continue;
+      }
+      // The token's warps are consecutive, the first holding x = 0 .. 31.  Two buffers, one barrier a turn: a
+      // buffer is written again only after the barrier that follows its reads.
+      if (lane == 0) {
+#pragma unroll
+        for (int u = 0; u < kP; ++u) red[buf][warp][u] = dot[u];
+      }
+      __syncthreads();
+      if (in_t && x < kP && j0 + x < a.k) {
+        float s = red[buf][warp][x];
+        for (int i = 1; i < cx / 32; ++i) s += red[buf][warp + i][x];
+        a.grad_w[t * a.k + j0 + x] = s;
+      }
+      buf ^= 1;
     }
-    __syncthreads();
-    if (in_t && x < 4 && j0 + x < a.k) {
-      float s = red[warp][x];  // this token's warps are consecutive, the first holding x = 0 .. 31
-      for (int i = 1; i < cx / 32; ++i) s += red[warp + i][x];
-      a.grad_w[t * a.k + j0 + x] = s;
-    }
-    __syncthreads();
   }
 }
 
@@ -745,15 +857,14 @@ int rows_shape(const char* what, rb::RowsArgs& a, int dtype, bool pads, int* rc)
   const bool vec = a.d % lanes == 0 && a.ld_src % lanes == 0 && a.ld_out % lanes == 0 && !unaligned(a.src, 16) &&
                    !unaligned(a.out, 16) && (a.extra == nullptr || (a.ld_extra % lanes == 0 && !unaligned(a.extra, 16)));
   const int per = vec ? lanes : 1;
+  // Threads to a token: a warp, and twice that as long as warps would stay idle and the row has vectors for them.
   const int64_t packs = (a.d + per - 1) / per;
+  const int64_t warps = (int64_t)rb_host::sm_budget(rb_host::current_device()) * 8 * rb::kRowsBlocksPerSm;
   a.cx = 32;
-  while (a.cx < 256 && a.cx < packs) a.cx <<= 1;
-  const int ny = 256 / a.cx;
-  a.token_blocks = (a.tokens + ny - 1) / ny;
-  if (pads) {  // about two thousand blocks for the rows to clear, at most 16 an expert
-    a.pad_slices = 2048 / (a.experts + 1);
+  while (a.cx < 256 && a.cx < packs && a.tokens * (a.cx / 32) < warps) a.cx <<= 1;
+  if (pads) {  // about two thousand pieces to clear, at most 16 an expert
+    a.pad_slices = 2048 / a.experts;
     if (a.pad_slices > 16) a.pad_slices = 16;
-    if (a.pad_slices < 1) a.pad_slices = 1;
   }
   *rc = RB_OK;
   return per;
@@ -761,16 +872,29 @@ int rows_shape(const char* what, rb::RowsArgs& a, int dtype, bool pads, int* rc)
 
 }  // namespace
 
-#define RB_ROWS_LAUNCH(kernel, grid)                                                                           \
-  do {                                                                                                         \
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);                                                  \
-    if (dtype == RB_DTYPE_BF16) {                                                                              \
-      if (per == 8) rb::kernel<__nv_bfloat16, 8><<<(unsigned)(grid), 256, 0, st>>>(a);                         \
-      else rb::kernel<__nv_bfloat16, 1><<<(unsigned)(grid), 256, 0, st>>>(a);                                  \
-    } else {                                                                                                   \
-      if (per == 4) rb::kernel<float, 4><<<(unsigned)(grid), 256, 0, st>>>(a);                                 \
-      else rb::kernel<float, 1><<<(unsigned)(grid), 256, 0, st>>>(a);                                          \
-    }                                                                                                          \
+// One wave of blocks, or as many as there are groups of tokens (and, with `pads`, pieces to clear) if that is
+// less.
+static unsigned rows_grid(const rb::RowsArgs& a, bool pads) {
+  const int64_t ny = 256 / a.cx, most = (int64_t)rb_host::sm_budget(rb_host::current_device()) * rb::kRowsBlocksPerSm;
+  int64_t want = (a.tokens + ny - 1) / ny;
+  if (pads && want < (int64_t)a.experts * a.pad_slices) want = (int64_t)a.experts * a.pad_slices;
+  return (unsigned)(want < most ? want : most);
+}
+
+#define RB_ROWS_LAUNCH_AS(kernel, T, vec)                                             \
+  (a.k <= 2 ? rb::kernel<T, vec, 2, rb::kRowsCols2><<<rows_grid(a, pads), 256, 0, st>>>(a) \
+            : rb::kernel<T, vec, 4, rb::kRowsCols4><<<rows_grid(a, pads), 256, 0, st>>>(a))
+#define RB_ROWS_LAUNCH(kernel, clears)                                                \
+  do {                                                                                \
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);                         \
+    constexpr bool pads = clears;                                                     \
+    if (dtype == RB_DTYPE_BF16) {                                                     \
+      if (per == 8) RB_ROWS_LAUNCH_AS(kernel, __nv_bfloat16, 8);                      \
+      else RB_ROWS_LAUNCH_AS(kernel, __nv_bfloat16, 1);                               \
+    } else {                                                                          \
+      if (per == 4) RB_ROWS_LAUNCH_AS(kernel, float, 4);                              \
+      else RB_ROWS_LAUNCH_AS(kernel, float, 1);                                       \
+    }                                                                                 \
   } while (0)
 
 extern "C" {
@@ -899,7 +1023,7 @@ int rb_nvfp4_token_dispatch(const void* x, int dtype, int64_t tokens, int64_t d,
       unaligned(counts, 8) || unaligned(offsets, 8))
     return route_failed(RB_ERR_ARG, "%s: null or misaligned pointer argument", what);
   if (!route_device(what)) return RB_ERR_DEVICE;
-  RB_ROWS_LAUNCH(token_dispatch_kernel, a.token_blocks + (int64_t)a.experts * a.pad_slices);
+  RB_ROWS_LAUNCH(token_dispatch_kernel, true);
   return route_launched(what);
 }
 
@@ -927,7 +1051,7 @@ int rb_nvfp4_token_combine(const void* y, int dtype, int64_t num_rows, int64_t d
   if (out == nullptr || rows == nullptr || (num_rows > 0 && y == nullptr))
     return route_failed(RB_ERR_ARG, "%s: null pointer argument", what);
   if (!route_device(what)) return RB_ERR_DEVICE;
-  RB_ROWS_LAUNCH(token_combine_kernel, a.token_blocks);
+  RB_ROWS_LAUNCH(token_combine_kernel, false);
   return route_launched(what);
 }
 
@@ -962,7 +1086,7 @@ int rb_nvfp4_token_combine_backward(const void* grad_y, int64_t ldg, const void*
       (tokens > 0 && (grad_y == nullptr || rows == nullptr || weights == nullptr || grad_weights == nullptr)))
     return route_failed(RB_ERR_ARG, "%s: null or misaligned pointer argument", what);
   if (!route_device(what)) return RB_ERR_DEVICE;
-  RB_ROWS_LAUNCH(token_combine_backward_kernel, a.token_blocks + (int64_t)a.experts * a.pad_slices);
+  RB_ROWS_LAUNCH(token_combine_backward_kernel, true);
   return route_launched(what);
 }
 
