@@ -7,49 +7,72 @@
 // the values in registers instead of from two more passes.
 #include "epilogue.cuh"
 
+#include <type_traits>
+
 namespace rb {
 
 // ---------------------------------------------------------------------------------------------
 // Dropout: y = residual + drop(x), flat over n elements
 // ---------------------------------------------------------------------------------------------
-// kVec: every pointer is 16-byte aligned.  A thread takes kUnroll groups of eight elements (one generator
-// call each) a step apart and loads them all before it computes: with one group at a time the kernel
-// waited on loads half of the time, at 4.0 TB/s.  Otherwise, and for the last n % 8 elements, elements go
-// one by one.
-constexpr int kUnroll = 2;
+// kVec: every pointer is 16-byte aligned, and a thread takes a group of eight elements (one generator call) a
+// turn, the next group's loads on their way while it computes.  Otherwise, and for the last n % 8 elements,
+// elements go one by one.
+// 16384 x 2048 bf16: 29 us (134 MB; a copy takes 23), with a residual 34 (201 MB, 5.9 TB/s); fp32 with a
+// residual 68 (5.9 TB/s).  Without a residual the generator's wide multiplies and xors bound it (the heavy half
+// of the FMA pipe 62% busy, the ALU 51%); more loads in flight (two or four groups a thread) cost occupancy
+// and time, 35 and 42 us.
+constexpr int kDropoutBlocksPerSm = 5;
 
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(256) dropout_kernel(const T* x, const T* residual, T* y, int64_t n,
+// Eight elements as loaded.
+template <typename T>
+struct Raw8 {
+  uint4 q[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) q[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void get(float2 (&v)[4]) const {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(q);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 2) v[j] = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+      else v[j] = make_float2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+    }
+  }
+};
+
+template <typename T, bool kVec, bool kResidual>
+__global__ void __launch_bounds__(256, kDropoutBlocksPerSm) dropout_kernel(const T* x, const T* residual, T* y, int64_t n,
                                                       const DropoutArgs d) {
-  const PhiloxKeys key = philox_keys<true>(d.seed);
+  const PhiloxKeys key = philox_keys(d.seed);
   const int64_t step = (int64_t)gridDim.x * blockDim.x, first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t groups = kVec ? n / 8 : 0;
-  for (int64_t g0 = first; g0 < groups; g0 += kUnroll * step) {
-    float2 v[kUnroll][4], r[kUnroll][4];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t g = g0 + u * step;
-      if (g < groups) {
-        Io<T>::load8(v[u], x + 8 * g);
-        if (residual != nullptr) Io<T>::load8(r[u], residual + 8 * g);
+  if (kVec && first < groups) {
+    Raw8<T> xn, rn;
+    xn.load(x + 8 * first);
+    if constexpr (kResidual) rn.load(residual + 8 * first);
+    for (int64_t g = first; g < groups; g += step) {
+      const Raw8<T> xc = xn, rc = rn;
+      if (g + step < groups) {
+        xn.load(x + 8 * (g + step));
+        if constexpr (kResidual) rn.load(residual + 8 * (g + step));
       }
-    }
+      float2 v[4];
+      xc.get(v);
+      if (d.seed != nullptr) dropout8(v, (uint64_t)g, key, d.below, d.scale);
+      if constexpr (kResidual) {
+        float2 r[4];
+        rc.get(r);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t g = g0 + u * step;
-      if (g >= groups) break;
-      if (d.seed != nullptr) dropout8(v[u], (uint64_t)g, key, d.below, d.scale);
-      if (residual != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[u][j] = __fadd2_rn(v[u][j], r[u][j]);
+        for (int j = 0; j < 4; ++j) v[j] = __fadd2_rn(v[j], r[j]);
       }
-      Io<T>::store8(y + 8 * g, v[u]);
+      Io<T>::store8(y + 8 * g, v);
     }
   }
   for (int64_t i = 8 * groups + first; i < n; i += step) {
     float u = Io<T>::load(x + i);
     if (d.seed != nullptr) u = dropout1(u, (uint64_t)i, key, d.below, d.scale);
-    Io<T>::store(y + i, residual != nullptr ? u + Io<T>::load(residual + i) : u);
+    Io<T>::store(y + i, kResidual ? u + Io<T>::load(residual + i) : u);
   }
 }
 
@@ -83,7 +106,7 @@ __global__ void __launch_bounds__(kBwdLanes* kBwdRows, kVec ? 4 : 2) epilogue_ba
   for (int j = 0; j < 4; ++j) sum[j] = both(0.0f);
   uint32_t m = 0;
   if (c < a.cols) {
-    const PhiloxKeys key = philox_keys<false>(a.drop.seed);
+    const PhiloxKeys key = philox_keys(a.drop.seed);
     if constexpr (kVec) {
 #pragma unroll 2
       for (int64_t r = r0 + ty; r < r1; r += kBwdRows) {
@@ -256,18 +279,23 @@ int rb_nvfp4_dropout(const void* x, const void* residual, int dtype, int64_t n, 
   if (!on_sm100(what)) return RB_ERR_DEVICE;
   const rb::DropoutArgs d = rb_host::dropout_args(p, seed);
   const bool vec = !misaligned16(x) && !misaligned16(y) && !misaligned16(residual);
-  const int64_t blocks = ((n + 7) / 8 + 255) / 256, most = (int64_t)8 * rb_host::sm_budget(rb_host::current_device());
+  const int64_t blocks = ((n + 7) / 8 + 255) / 256;
+  const int64_t most = (int64_t)rb::kDropoutBlocksPerSm * rb_host::sm_budget(rb_host::current_device());
   const unsigned grid = (unsigned)(blocks < most ? blocks : most);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == RB_DTYPE_BF16) {
-    using T = __nv_bfloat16;
+  const auto launch = [&](auto t, auto v) {
+    using T = decltype(t);
+    constexpr bool kVec = decltype(v)::value;
     const T *px = reinterpret_cast<const T*>(x), *pr = reinterpret_cast<const T*>(residual);
-    if (vec) rb::dropout_kernel<T, true><<<grid, 256, 0, st>>>(px, pr, reinterpret_cast<T*>(y), n, d);
-    else rb::dropout_kernel<T, false><<<grid, 256, 0, st>>>(px, pr, reinterpret_cast<T*>(y), n, d);
+    if (pr != nullptr) rb::dropout_kernel<T, kVec, true><<<grid, 256, 0, st>>>(px, pr, reinterpret_cast<T*>(y), n, d);
+    else rb::dropout_kernel<T, kVec, false><<<grid, 256, 0, st>>>(px, pr, reinterpret_cast<T*>(y), n, d);
+  };
+  if (dtype == RB_DTYPE_BF16) {
+    if (vec) launch(__nv_bfloat16(), std::true_type());
+    else launch(__nv_bfloat16(), std::false_type());
   } else {
-    const float *px = reinterpret_cast<const float*>(x), *pr = reinterpret_cast<const float*>(residual);
-    if (vec) rb::dropout_kernel<float, true><<<grid, 256, 0, st>>>(px, pr, reinterpret_cast<float*>(y), n, d);
-    else rb::dropout_kernel<float, false><<<grid, 256, 0, st>>>(px, pr, reinterpret_cast<float*>(y), n, d);
+    if (vec) launch(float(), std::true_type());
+    else launch(float(), std::false_type());
   }
   return launched(what);
 }

@@ -26,14 +26,11 @@ struct DropoutArgs {
   float scale;
 };
 
-// The ten rounds' keys, which depend on the seed alone.  kHold: they are kept in 20 registers (the empty
-// asm hides that they could be computed again), sparing every call 18 additions, about a fifth of its
-// integer work; without it the compiler adds them up in each call.
+// The ten rounds' keys, which depend on the seed alone.
 struct PhiloxKeys {
   uint32_t k0[10], k1[10];
 };
 
-template <bool kHold>
 __device__ __forceinline__ PhiloxKeys philox_keys(const int64_t* seed) {
   PhiloxKeys k;
   const uint64_t s = seed != nullptr ? static_cast<uint64_t>(__ldg(reinterpret_cast<const long long*>(seed))) : 0;
@@ -41,7 +38,6 @@ __device__ __forceinline__ PhiloxKeys philox_keys(const int64_t* seed) {
   for (int r = 0; r < 10; ++r) {
     k.k0[r] = static_cast<uint32_t>(s) + r * 0x9E3779B9u;
     k.k1[r] = static_cast<uint32_t>(s >> 32) + r * 0xBB67AE85u;
-    if constexpr (kHold) asm("" : "+r"(k.k0[r]), "+r"(k.k1[r]));
   }
   return k;
 }

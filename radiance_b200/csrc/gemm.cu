@@ -1041,7 +1041,7 @@ __device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, cons
   uint64_t* bars = &sm.res_full[2 * ew];
   float* bias_sm = sm.bias[ew];
   const bool residual = g.has_residual != 0, preact = g.has_preact != 0;
-  const PhiloxKeys key = philox_keys<false>(g.drop.seed);
+  const PhiloxKeys key = philox_keys(g.drop.seed);
   const uint32_t sw = (uint32_t)(lane & 7), lane_row = (uint32_t)lane * 128u;
   const uint64_t policy = policy_evict_first();
   float alpha = 1.0f;

@@ -17,7 +17,11 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import _trace
-from .quantize import NVFP4Tensor, _require_cuda, _stream_ptr
+from .quantize import NVFP4Tensor, _require_cuda
+
+# The current stream's handle without the Stream object around it (2 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 _DTYPES = {torch.bfloat16: _lib.RB_DTYPE_BF16, torch.float32: _lib.RB_DTYPE_F32}
 
@@ -31,11 +35,12 @@ def _dtype_of(x: torch.Tensor, what: str) -> int:
 
 def _call(what: str, device: torch.device, fn, *args) -> None:
     """One C call (its stream argument appended) with ``device`` current, and its error raised."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, _stream_ptr(device))
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _stream_ptr(device))
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, what)
 
