@@ -13,7 +13,7 @@
 
 namespace rb {
 
-constexpr int kRouteThreads = 256;
+constexpr int kRouteThreads = 512;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kMaxExperts = 256;   // the grouped GEMM's group limit
 constexpr int kMaxTopK = 32;       // one lane keeps one pick
@@ -181,21 +181,42 @@ __device__ __forceinline__ void plan_block(const RouteArgs& a, int64_t c0, int64
   }
 }
 
+// The best of a group's (key, expert) candidates: the largest key, ties to the lower expert.
+template <int LPT>
+__device__ __forceinline__ void group_best(uint32_t& key, int& expert) {
+  if constexpr (LPT == 32) {  // whole warps have reductions in hardware
+    const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, key);
+    expert = (int)__reduce_min_sync(0xFFFFFFFFu, key == m ? (uint32_t)expert : 0x7FFFFFFFu);
+    key = m;
+  } else {
+#pragma unroll
+    for (int o = LPT / 2; o > 0; o >>= 1) {
+      const uint32_t ok = __shfl_xor_sync(0xFFFFFFFFu, key, o);
+      const int oe = __shfl_xor_sync(0xFFFFFFFFu, expert, o);
+      if (ok > key || (ok == key && oe < expert)) key = ok, expert = oe;
+    }
+  }
+}
+
 // One block takes `chunk` consecutive tokens.  LPT lanes hold one token's logits, ITEMS experts to a
 // lane (expert e sits in lane e % LPT), so a warp works on 32 / LPT tokens and its loads of a row are
-// contiguous.  First the tokens: softmax, the k picks one maximum at a time, weights, and each lane's
-// sums of its experts' probabilities.  Then the pairs, from shared memory: each warp ranks a run of
-// them among the pairs of the same expert (match_any gives the lanes with the same pick), the warps'
-// counts are scanned, and the block's ranks and counts go out for plan_block.
-// 16384 x 8, k = 2: the pass reads 0.5 MB; what it costs is the launch and one block's latency, so
-// the tokens are spread over one block per SM.
+// contiguous.  First the tokens: softmax, the k picks one maximum at a time (a lane looks through its own
+// experts again only when one of them was picked), weights, and each lane's sums of its experts' probabilities.
+// Then the pairs, from shared memory: each warp ranks a run of them among the pairs of the same expert
+// (match_any gives the lanes with the same pick), the warps' counts are scanned, and the block's ranks and
+// counts go out for plan_block.
+// What this costs is latency, a launch's and a block's: the tokens are spread over one block per SM, and a
+// block of sixteen warps goes through its share in a step or two.  With plan_block, 16384 x 8, k = 2: ROUTE_A;
+// 4099 x 160, k = 6: ROUTE_B (eight warps, five shuffles for each of two values a pick: 12.5 and 35 us).
 template <typename T, int LPT, int ITEMS>
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a) {
   constexpr int kGroups = kRouteThreads / LPT;
   __shared__ int16_t pair[kMaxPairs];
   __shared__ uint16_t rank[kMaxPairs];
-  __shared__ int32_t whist[kRouteWarps][kMaxExperts];
-  __shared__ float wp[kRouteWarps][LPT * ITEMS];
+  __shared__ union {
+    float p[kRouteWarps][kMaxExperts];    // sums of probabilities, then
+    int32_t n[kRouteWarps][kMaxExperts];  // counts of pairs
+  } per_warp;
   __shared__ int32_t wn[kRouteWarps];
   __shared__ PlanSmem plan;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -222,6 +243,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a)
       nan |= x[i] != x[i];
     }
     m = group_max<LPT>(m);
+    const float top = m;
     if (nan) m = NAN;  // this lane's exponentials become NaN, and with them the sum
     float z = 0.0f, p[ITEMS];
 #pragma unroll
@@ -231,24 +253,29 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a)
       z += p[i];
     }
     z = group_sum<LPT>(z);
+    uint32_t lane_key = 0;  // the best of this lane's experts that are left
+    int lane_best = 0x7FFFFFFF;
+    const auto look = [&]() {
+      lane_key = 0;
+      lane_best = 0x7FFFFFFF;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+        if (key[i] > lane_key) lane_key = key[i], lane_best = i * LPT + gl;
+    };
+    look();
     int mine = -1;  // lane j of the group keeps pick j
     for (int j = 0; j < a.k; ++j) {
-      uint32_t bk = 0;
-      int be = 0x7FFFFFFF;
-#pragma unroll
-      for (int i = 0; i < ITEMS; ++i)
-        if (key[i] > bk) bk = key[i], be = i * LPT + gl;
-#pragma unroll
-      for (int o = LPT / 2; o > 0; o >>= 1) {
-        const uint32_t ok = __shfl_xor_sync(0xFFFFFFFFu, bk, o);
-        const int oe = __shfl_xor_sync(0xFFFFFFFFu, be, o);
-        if (ok > bk || (ok == bk && oe < be)) bk = ok, be = oe;
-      }
-      if (bk == 0) be = -1;  // nothing selectable is left
+      uint32_t bk = lane_key;
+      int be = lane_best;
+      group_best<LPT>(bk, be);
+      if (bk == 0) be = -1;  // nothing selectable is left (the loop goes on: other groups of the warp need it)
       if (gl == j) mine = be;
+      if (be == lane_best) {
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i)
-        if (be == i * LPT + gl) key[i] = 0;
+        for (int i = 0; i < ITEMS; ++i)
+          if (be == i * LPT + gl) key[i] = 0;
+        look();
+      }
     }
     const bool routed = __shfl_sync(0xFFFFFFFFu, mine, lane & ~(LPT - 1)) >= 0;
     if (routed) {
@@ -266,9 +293,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a)
       const float sum = group_sum<LPT>(w);
       w = mine >= 0 ? w / sum : 0.0f;
     } else {
-      // x - m in this lane may be NaN only through m: the group's maximum is taken again without it.
-      const float mm = group_max<LPT>(nan ? -INFINITY : m);
-      w = mine >= 0 ? expf(xs - mm) / z : 0.0f;
+      w = mine >= 0 ? expf(xs - top) / z : 0.0f;
     }
     if (t < t1 && gl < a.k) {
       a.weights[t * a.k + gl] = w;
@@ -281,13 +306,25 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a)
   for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll
     for (int o = 16; o >= LPT; o >>= 1) acc[i] += __shfl_xor_sync(0xFFFFFFFFu, acc[i], o);
-    if (lane < LPT) wp[warp][i * LPT + gl] = acc[i];
+    if (lane < LPT && i * LPT + gl < kMaxExperts) per_warp.p[warp][i * LPT + gl] = acc[i];
   }
   nrouted = __reduce_add_sync(0xFFFFFFFFu, nrouted);
   if (lane == 0) wn[warp] = nrouted;
-  for (int i = lane; i < a.experts; i += 32) whist[warp][i] = 0;
+  __syncthreads();
+  if ((int)threadIdx.x < a.experts) {
+    float ps = 0.0f;
+    for (int w = 0; w < kRouteWarps; ++w) ps += per_warp.p[w][threadIdx.x];
+    a.psum[(int64_t)blockIdx.x * a.experts + threadIdx.x] = ps;
+  }
+  if (threadIdx.x == 0) {
+    int n = 0;
+    for (int w = 0; w < kRouteWarps; ++w) n += wn[w];
+    a.nrouted[blockIdx.x] = n;
+  }
   __syncthreads();
   // Ranks within this warp's run of pairs.
+  for (int i = lane; i < a.experts; i += 32) per_warp.n[warp][i] = 0;
+  __syncwarp();
   const int pairs = t1 > t0 ? (int)((t1 - t0) * a.k) : 0;
   const int run = ((pairs + kRouteWarps - 1) / kRouteWarps + 31) & ~31;
   const int p0 = warp * run, p1 = min(pairs, p0 + run);
@@ -296,36 +333,29 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a)
     const int e = i < p1 ? (int)pair[i] : -1;
     const uint32_t same = __match_any_sync(0xFFFFFFFFu, e);
     int before = 0;
-    if (e >= 0) before = whist[warp][e];
+    if (e >= 0) before = per_warp.n[warp][e];
     __syncwarp();
     if (e >= 0) {
       rank[i] = (uint16_t)(before + __popc(same & ((1u << lane) - 1u)));
-      if ((same >> lane) == 1u) whist[warp][e] = before + __popc(same);  // the last lane of its kind
+      if ((same >> lane) == 1u) per_warp.n[warp][e] = before + __popc(same);  // the last lane of its kind
     }
     __syncwarp();
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
+  if ((int)threadIdx.x < a.experts) {
+    const int e = threadIdx.x;
     int sum = 0;
-    float ps = 0.0f;
     for (int w = 0; w < kRouteWarps; ++w) {
-      const int h = whist[w][e];
-      whist[w][e] = sum;  // pairs of this expert in earlier warps
+      const int h = per_warp.n[w][e];
+      per_warp.n[w][e] = sum;  // pairs of this expert in earlier warps
       sum += h;
-      ps += wp[w][e];
     }
     a.hist[(int64_t)blockIdx.x * a.experts + e] = sum;
-    a.psum[(int64_t)blockIdx.x * a.experts + e] = ps;
-  }
-  if (threadIdx.x == 0) {
-    int n = 0;
-    for (int w = 0; w < kRouteWarps; ++w) n += wn[w];
-    a.nrouted[blockIdx.x] = n;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < pairs; i += kRouteThreads) {
     const int e = pair[i];
-    if (e >= 0) a.rows[t0 * a.k + i] = whist[i / run][e] + rank[i];
+    if (e >= 0) a.rows[t0 * a.k + i] = per_warp.n[i / run][e] + rank[i];
   }
   if (gridDim.x == 1) {  // few tokens: this block finishes the plan itself
     __syncthreads();
@@ -825,7 +855,9 @@ void route_shape(int experts, F&& f) {
   else if (l == 16) f(integral_constant<int, 16>(), integral_constant<int, 1>());
   else if (experts <= 32) f(integral_constant<int, 32>(), integral_constant<int, 1>());
   else if (experts <= 64) f(integral_constant<int, 32>(), integral_constant<int, 2>());
+  else if (experts <= 96) f(integral_constant<int, 32>(), integral_constant<int, 3>());
   else if (experts <= 128) f(integral_constant<int, 32>(), integral_constant<int, 4>());
+  else if (experts <= 192) f(integral_constant<int, 32>(), integral_constant<int, 6>());
   else f(integral_constant<int, 32>(), integral_constant<int, 8>());
 }
 
