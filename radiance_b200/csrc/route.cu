@@ -37,7 +37,7 @@ struct RouteArgs {
   int64_t chunk;        // tokens per block
   int64_t blocks;
   // scratch, per block: pairs of each expert, sums of each expert's probability, routed tokens
-  int32_t* hist;        // blocks x experts
+  uint16_t* hist;       // blocks x experts (a block has at most kMaxPairs pairs)
   float* psum;          // blocks x experts
   int32_t* nrouted;     // blocks
 };
@@ -97,23 +97,33 @@ struct PlanSmem {
 
 // The second half of routing, by one block: the totals of every expert over all blocks' counts,
 // then the final rows of the pairs of chunks [c0, c1); with `summary`, also counts, offsets and loss.
-// Threads (s, e) = (tid / ep, tid % ep) share the blocks' counts of expert e, ep the power of two >= experts.
+// As many threads as fit share an expert: thread s * experts + e adds the counts of blocks s, s + ns, ...,
+// kAhead loads in flight, since nothing but their latency costs time here (one after the other: 14 us for 129
+// blocks' counts of 160 experts).
 __device__ __forceinline__ void plan_block(const RouteArgs& a, int64_t c0, int64_t c1, bool summary, PlanSmem& sm) {
-  int ep = 1;
-  while (ep < a.experts) ep <<= 1;
-  const int e = (int)threadIdx.x & (ep - 1), s = (int)threadIdx.x / ep, ns = kRouteThreads / ep;
+  constexpr int kAhead = 16;
+  const int ns = kRouteThreads / a.experts, s = (int)threadIdx.x / a.experts;
+  const int e = (int)threadIdx.x - s * a.experts;
   int32_t tot = 0, pre = 0;
   float ps = 0.0f;
-  if (e < a.experts) {
-#pragma unroll 8
-    for (int64_t b = s; b < a.blocks; b += ns) {
-      const int32_t h = __ldcg(a.hist + b * a.experts + e);
-      tot += h;
-      if (b < c0) pre += h;
-    }
-    if (summary) {
-#pragma unroll 8
-      for (int64_t b = s; b < a.blocks; b += ns) ps += __ldcg(a.psum + b * a.experts + e);
+  if (s < ns) {
+    // From chunk c0 on and round to it: started at chunk 0 by every block, they all ask for the same lines at
+    // the same time.
+    for (int64_t i0 = s; i0 < a.blocks; i0 += kAhead * ns) {
+      int32_t h[kAhead];
+      float p[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int64_t i = i0 + u * ns, b = i + c0 < a.blocks ? i + c0 : i + c0 - a.blocks;
+        h[u] = i < a.blocks ? (int32_t)__ldcg(a.hist + b * a.experts + e) : 0;
+        p[u] = summary && i < a.blocks ? __ldcg(a.psum + b * a.experts + e) : 0.0f;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        tot += h[u];
+        if (i0 + u * ns + c0 >= a.blocks) pre += h[u];
+        ps += p[u];
+      }
     }
   }
   sm.tot[threadIdx.x] = tot;
@@ -125,9 +135,9 @@ __device__ __forceinline__ void plan_block(const RouteArgs& a, int64_t c0, int64
   double p = 0.0;
   if (x < a.experts) {
     for (int i = 0; i < ns; ++i) {
-      total += sm.tot[i * ep + x];
-      prefix += sm.pre[i * ep + x];
-      p += sm.ps[i * ep + x];
+      total += sm.tot[i * a.experts + x];
+      prefix += sm.pre[i * a.experts + x];  // 0 in a summary, which starts at chunk 0
+      p += sm.ps[i * a.experts + x];
     }
   }
   const int64_t padded = (total + kGroupAlign - 1) / kGroupAlign * kGroupAlign;
@@ -169,9 +179,19 @@ __device__ __forceinline__ void plan_block(const RouteArgs& a, int64_t c0, int64
   __syncthreads();
   for (int64_t ch = c0; ch < c1; ++ch) {
     const int64_t i0 = ch * a.chunk * a.k, i1 = min(a.tokens, (ch + 1) * a.chunk) * a.k;
-    for (int64_t i = i0 + x; i < i1; i += kRouteThreads) {
-      const int32_t pick = __ldcg(a.picks + i);
-      a.rows[i] = pick < 0 ? -1 : (int32_t)(sm.base[pick] + __ldcg(a.rows + i));
+    for (int64_t i = i0 + x; i < i1; i += 4 * kRouteThreads) {
+      int32_t pick[4], rank[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t at = i + u * kRouteThreads;
+        pick[u] = at < i1 ? __ldcg(a.picks + at) : -1;
+        rank[u] = at < i1 ? __ldcg(a.rows + at) : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t at = i + u * kRouteThreads;
+        if (at < i1) a.rows[at] = pick[u] < 0 ? -1 : (int32_t)(sm.base[pick[u]] + rank[u]);
+      }
     }
     if (ch + 1 < c1) {
       __syncthreads();
@@ -206,8 +226,8 @@ __device__ __forceinline__ void group_best(uint32_t& key, int& expert) {
 // (match_any gives the lanes with the same pick), the warps' counts are scanned, and the block's ranks and
 // counts go out for plan_block.
 // What this costs is latency, a launch's and a block's: the tokens are spread over one block per SM, and a
-// block of sixteen warps goes through its share in a step or two.  With plan_block, 16384 x 8, k = 2: ROUTE_A;
-// 4099 x 160, k = 6: ROUTE_B (eight warps, five shuffles for each of two values a pick: 12.5 and 35 us).
+// block of sixteen warps goes through its share in a step or two.  With plan_block, 16384 x 8, k = 2: 10.7 us;
+// 4099 x 160, k = 6: 18.7 us (eight warps, five shuffles for each of two values a pick: 12.5 and 35 us).
 template <typename T, int LPT, int ITEMS>
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a) {
   constexpr int kGroups = kRouteThreads / LPT;
@@ -350,12 +370,12 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a)
       per_warp.n[w][e] = sum;  // pairs of this expert in earlier warps
       sum += h;
     }
-    a.hist[(int64_t)blockIdx.x * a.experts + e] = sum;
+    a.hist[(int64_t)blockIdx.x * a.experts + e] = (uint16_t)sum;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < pairs; i += kRouteThreads) {
     const int e = pair[i];
-    if (e >= 0) a.rows[t0 * a.k + i] = per_warp.n[i / run][e] + rank[i];
+    a.rows[t0 * a.k + i] = e >= 0 ? per_warp.n[i / run][e] + rank[i] : 0;
   }
   if (gridDim.x == 1) {  // few tokens: this block finishes the plan itself
     __syncthreads();
@@ -830,14 +850,14 @@ int route_lanes(int experts) {
   return l;
 }
 
-// Tokens per block: one block per SM, whole steps of the block's token groups, and no more pairs than
+// Tokens per block: the same for every SM, in whole steps of the block's token groups, and no more pairs than
 // its shared memory holds.
 int64_t route_chunk(int64_t tokens, int experts, int k) {
   const int groups = rb::kRouteThreads / route_lanes(experts);
-  const int sms = rb_host::sm_budget(rb_host::current_device());
-  int64_t c = (tokens + sms - 1) / sms;
+  const int64_t sms = rb_host::sm_budget(rb_host::current_device());
   const int64_t most = rb::kMaxPairs / k;
-  if (c > most) c = most;
+  const int64_t turns = (tokens + sms * most - 1) / (sms * most);  // blocks per SM
+  int64_t c = turns > 0 ? (tokens + sms * turns - 1) / (sms * turns) : 1;
   c = (c + groups - 1) / groups * groups;
   if (c > most) c = most;
   return c < 1 ? 1 : c;
@@ -935,7 +955,7 @@ size_t rb_nvfp4_route_workspace(int64_t tokens, int64_t experts, int k) {
   if (tokens < 0 || experts < 1 || experts > rb::kMaxExperts || k < 1 || k > rb::kMaxTopK) return 0;
   const int64_t chunk = route_chunk(tokens, (int)experts, k);
   const int64_t blocks = tokens > 0 ? (tokens + chunk - 1) / chunk : 1;
-  return (size_t)(blocks * (2 * experts + 1)) * 4;
+  return (size_t)(blocks * (6 * experts + 4));
 }
 
 int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
@@ -969,9 +989,9 @@ int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t expert
   a.routed = routed;
   a.chunk = route_chunk(tokens, a.experts, k);
   a.blocks = tokens > 0 ? (tokens + a.chunk - 1) / a.chunk : 1;
-  a.hist = reinterpret_cast<int32_t*>(workspace);
-  a.psum = reinterpret_cast<float*>(a.hist + a.blocks * experts);
+  a.psum = reinterpret_cast<float*>(workspace);
   a.nrouted = reinterpret_cast<int32_t*>(a.psum + a.blocks * experts);
+  a.hist = reinterpret_cast<uint16_t*>(a.nrouted + a.blocks);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   route_shape(a.experts, [&](auto l, auto i) {
     if (dtype == RB_DTYPE_BF16)
