@@ -177,6 +177,18 @@ def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     return lda != ldb or at < width or at + width > lda
 
 
+def _operand(q: NVFP4Tensor, device: torch.device, what: str) -> None:
+    """Refuses an operand whose tensors the kernel would read past or cannot read."""
+    rows, k2 = q.packed.shape
+    if q.packed.device != device or q.scale.device != device or q.global_scale.device != device:
+        raise ValueError(f"{what}: all parts of both operands must be on {device}")
+    if not q.packed.is_contiguous() or not q.scale.is_contiguous() or q.packed.element_size() != 1 \
+            or q.scale.element_size() != 1 or q.scale.numel() < (rows // 128) * (k2 // 32) * 512 \
+            or q.global_scale.dtype != torch.float32 or q.global_scale.numel() != 1:
+        raise ValueError(f"{what}: an operand of {rows} x {2 * k2} needs contiguous packed codes, its block scales and "
+                         "one fp32 global scale")
+
+
 def epilogue_mm(a: NVFP4Tensor, b: NVFP4Tensor, *, bias: torch.Tensor | None = None, activation: str | None = None,
                 dropout_p: float = 0.0, seed: torch.Tensor | int | None = None, residual: torch.Tensor | None = None,
                 out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None, save_preact: bool = False
@@ -191,14 +203,16 @@ def epilogue_mm(a: NVFP4Tensor, b: NVFP4Tensor, *, bias: torch.Tensor | None = N
     ``epilogue_backward`` takes.
     """
     what = "nvfp4.epilogue_mm"
-    _require_cuda(a.packed, what)
-    dev = a.packed.device
-    ap, asc = a.packed.view(torch.uint8), a.scale.view(torch.uint8)
-    bp, bsc = b.packed.view(torch.uint8), b.scale.view(torch.uint8)
+    ap, bp = a.packed, b.packed
+    _require_cuda(ap, what)
+    dev = ap.device
     (m, k2), (n, k2b) = ap.shape, bp.shape
     if k2 != k2b:
         raise ValueError(f"{what}: contraction mismatch {2 * k2} vs {2 * k2b}")
-    if out_dtype not in _DTYPES:
+    _operand(a, dev, what)
+    _operand(b, dev, what)
+    out_code = _DTYPES.get(out_dtype)
+    if out_code is None:
         raise ValueError(f"{what}: unsupported output dtype {out_dtype} (bf16 or fp32)")
     act, p = _activation_code(activation, what), _probability(dropout_p, what)
     seed = _seed_tensor(seed, dev, what) if p > 0.0 else None
@@ -209,11 +223,12 @@ def epilogue_mm(a: NVFP4Tensor, b: NVFP4Tensor, *, bias: torch.Tensor | None = N
         if bias.dtype not in _DTYPES:
             bias = bias.to(torch.float32)
         bias = bias.contiguous()
-        if bias.data_ptr() % 16:  # the epilogue reads the bias in 16-byte vectors
+        if bias.data_ptr() % 16:  # the epilogue reads the bias in vectors
             bias = bias.clone()
         bias_code = _DTYPES[bias.dtype]
     if residual is not None:
         _like("residual", residual, (m, n), out_dtype, dev, what)
+    ldo = ldr = n
     if out is None:
         out = torch.empty(m, n, dtype=out_dtype, device=dev)
     else:
@@ -223,15 +238,17 @@ def epilogue_mm(a: NVFP4Tensor, b: NVFP4Tensor, *, bias: torch.Tensor | None = N
         if residual is not None and _share_memory(out, _rows(residual)[0]) and not (
                 out.data_ptr() == residual.data_ptr() and out.stride() == residual.stride()):
             raise ValueError(f"{what}: out overlaps the residual without being the residual")
+        ldo = _rows(out)[1]
     if residual is not None:
         residual = _tma_rows(residual)
+        ldr = _rows(residual)[1]
     z = torch.empty(m, n, dtype=out_dtype, device=dev) if save_preact else None
     tok = _trace.begin("gemm", 4.0 * m * n * k2)
-    _call(what, dev, _lib.load().rb_nvfp4_gemm_epilogue, ap.data_ptr(), asc.data_ptr(), bp.data_ptr(), bsc.data_ptr(),
-          m, n, 2 * k2, a.global_scale.data_ptr(), b.global_scale.data_ptr(), None if bias is None else bias.data_ptr(),
-          bias_code, act, p, None if seed is None else seed.data_ptr(),
-          None if residual is None else residual.data_ptr(), n if residual is None else _rows(residual)[1],
-          None if z is None else z.data_ptr(), n, out.data_ptr(), _DTYPES[out_dtype], _rows(out)[1])
+    _call(what, dev, _lib.load().rb_nvfp4_gemm_epilogue, ap.data_ptr(), a.scale.data_ptr(), bp.data_ptr(),
+          b.scale.data_ptr(), m, n, 2 * k2, a.global_scale.data_ptr(), b.global_scale.data_ptr(),
+          None if bias is None else bias.data_ptr(), bias_code, act, p, None if seed is None else seed.data_ptr(),
+          None if residual is None else residual.data_ptr(), ldr, None if z is None else z.data_ptr(), n,
+          out.data_ptr(), out_code, ldo)
     _trace.end(tok)
     return (out, z) if save_preact else out
 
@@ -265,12 +282,14 @@ def epilogue_backward(grad_y: torch.Tensor, preact: torch.Tensor | None = None, 
         if seed is None:
             raise ValueError(f"{what}: dropout needs the forward call's seed")
         seed = _seed_tensor(seed, dev, what)
+    ldo = cols
     if out is None:
         out = torch.empty(rows, cols, dtype=grad_y.dtype, device=dev)
     else:
         _like("out", out, (rows, cols), grad_y.dtype, dev, what)
         if _rows(out)[0] is not out:
             raise ValueError(f"{what}: out must have contiguous rows")
+        ldo = _rows(out)[1]
     gs = torch.empty((), dtype=torch.float32, device=dev)
     sums = torch.empty(cols, dtype=torch.float32, device=dev) if bias_grad else None
     lib = _lib.load()
@@ -278,7 +297,7 @@ def epilogue_backward(grad_y: torch.Tensor, preact: torch.Tensor | None = None, 
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     tok = _trace.begin("epilogue", rows * cols * grad_y.element_size() * (2 + (z is not None)))
     _call(what, dev, lib.rb_nvfp4_epilogue_backward, grad_y.data_ptr(), ldg, None if z is None else z.data_ptr(), ldz,
-          code, rows, cols, act, p, seed.data_ptr() if p > 0.0 else None, out.data_ptr(), _rows(out)[1], gs.data_ptr(),
+          code, rows, cols, act, p, seed.data_ptr() if p > 0.0 else None, out.data_ptr(), ldo, gs.data_ptr(),
           None if sums is None else sums.data_ptr(), ws.data_ptr(), need)
     _trace.end(tok)
     return out, gs, sums

@@ -258,6 +258,14 @@ def test_mm_refusals(nv):
     res = _rand(256, 256, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="contraction"):
         nv.epilogue_mm(qa, short)
+    for bad in (qa.packed.view(torch.uint8)[:, ::2].view(torch.uint8), qa.packed):
+        scale = qa.scale[:100] if bad is qa.packed else qa.scale
+        with pytest.raises(ValueError, match="contraction|needs contiguous"):
+            nv.epilogue_mm(nv.NVFP4Tensor(bad, scale, qa.global_scale), qb)
+    with pytest.raises(ValueError, match="needs contiguous"):
+        nv.epilogue_mm(nv.NVFP4Tensor(qa.packed, qa.scale, qa.global_scale.double()), qb)
+    with pytest.raises(ValueError, match="must be on"):
+        nv.epilogue_mm(qa, nv.NVFP4Tensor(qb.packed, qb.scale, qb.global_scale.cpu()))
     with pytest.raises(ValueError, match="output dtype"):
         nv.epilogue_mm(qa, qb, out_dtype=torch.float16)
     with pytest.raises(ValueError, match="activation"):
