@@ -93,7 +93,10 @@ struct EpilogueBwdArgs {
 constexpr int kBwdLanes = 32;  // threads along a row, 8 columns each: a block covers 256 columns
 constexpr int kBwdRows = 8;    // rows a block reads at once
 constexpr int kBwdBlocksPerSm = 3;
-constexpr int kBwdBatch = 3;   // rows of a thread in flight
+
+// Rows of a thread in flight: three of bf16, two of fp32 (a third would be spilled).
+template <typename T>
+constexpr int kBwdBatchOf = sizeof(T) == 2 ? 3 : 2;
 
 // 16384 x 5632 bf16 with the bias gradient: without an activation 64 us, relu^2 91, silu 90, GELU 101, against 57 and
 // 86 for the bytes at the copy's rate.  Four blocks to an SM with a row or two in flight: 69 to 77, 90 to 96, 97
@@ -113,6 +116,7 @@ __global__ void __launch_bounds__(kBwdLanes* kBwdRows, kBwdBlocksPerSm) epilogue
   if (c < a.cols) {
     const PhiloxKeys key = philox_keys(a.drop.seed);
     if constexpr (kVec) {
+      constexpr int kBwdBatch = kBwdBatchOf<T>;
       for (int64_t rb = r0 + ty; rb < r1; rb += kBwdBatch * kBwdRows) {
         Raw8<T> graw[kBwdBatch], zraw[kBwdBatch];
 #pragma unroll
