@@ -91,7 +91,13 @@ __device__ __forceinline__ float ex2_approx(float x) {  // within 2 ulp; large x
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 relu2(float2 z) { return make_float2(max_nan(z.x, 0.0f), max_nan(z.y, 0.0f)); }
 __device__ __forceinline__ float2 rcp2(float2 x) { return make_float2(rcp_approx(x.x), rcp_approx(x.y)); }
 __device__ __forceinline__ float2 ex2_2(float2 x) { return make_float2(ex2_approx(x.x), ex2_approx(x.y)); }
 
@@ -114,14 +120,15 @@ __device__ __forceinline__ float2 gelu_tanh_sigmoid2(float2 z) {
 // Hastings' formula (C. Hastings, "Approximations for Digital Computers", 1955, sheet 45; 7.1.26 of
 // Abramowitz and Stegun): erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), within
 // 1.5e-7 for x >= 0.  Halved here.  One reciprocal and one exponential, with e shared by the derivative, where
-// erff takes a branch and some 25 instructions more.  `az` is |z| held below 128, where q is 0.
+// erff takes a branch and some 25 instructions more.  `nz` is -|z| held above -128, where q is 0; for a NaN it is
+// -128, and the NaN comes through e.
 struct NormalTail {
-  float2 az, q, e;
+  float2 nz, q, e;
 };
 __device__ __forceinline__ NormalTail normal_tail2(float2 z) {
   NormalTail n;
-  n.az = make_float2(fminf(fabsf(z.x), 128.0f), fminf(fabsf(z.y), 128.0f));
-  const float2 t = rcp2(__ffma2_rn(n.az, both(0.3275911f * 0.70710678118654752f), both(1.0f)));
+  n.nz = make_float2(fmaxf(-fabsf(z.x), -128.0f), fmaxf(-fabsf(z.y), -128.0f));
+  const float2 t = rcp2(__ffma2_rn(n.nz, both(-0.3275911f * 0.70710678118654752f), both(1.0f)));
   float2 p = __ffma2_rn(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
   p = __ffma2_rn(t, p, both(0.5f * 1.421413741f));
   p = __ffma2_rn(t, p, both(0.5f * -0.284496736f));
@@ -133,16 +140,15 @@ __device__ __forceinline__ NormalTail normal_tail2(float2 z) {
 
 template <int kAct>
 __device__ __forceinline__ float2 act_value2(float2 z) {
-  if constexpr (kAct == RB_ACT_RELU) return make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y);  // NaN stays
+  if constexpr (kAct == RB_ACT_RELU) return relu2(z);
   else if constexpr (kAct == RB_ACT_RELU2) {
-    const float2 r = make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y);
+    const float2 r = relu2(z);
     return __fmul2_rn(r, r);
   } else if constexpr (kAct == RB_ACT_SILU) return __fmul2_rn(z, sigmoid2(z));
   else if constexpr (kAct == RB_ACT_GELU) {
     // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
     const NormalTail n = normal_tail2(z);
-    const float2 pos = make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y);
-    return __ffma2_rn(make_float2(-n.az.x, -n.az.y), n.q, pos);
+    return __ffma2_rn(n.nz, n.q, make_float2(fmaxf(z.x, 0.0f), fmaxf(z.y, 0.0f)));
   } else if constexpr (kAct == RB_ACT_GELU_TANH) return __fmul2_rn(z, gelu_tanh_sigmoid2(z));
   else return z;
 }
