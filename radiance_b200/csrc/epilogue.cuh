@@ -106,15 +106,13 @@ constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kGeluA = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluB = 0.044715f;
 
-__device__ __forceinline__ float2 sigmoid2(float2 z) {
-  return rcp2(__fadd2_rn(ex2_2(__fmul2_rn(z, both(-kLog2e))), both(1.0f)));
+// silu(z) = z / (1 + 2^x) for x = -log2(e) z, and the tanh form of GELU, 0.5 z (1 + tanh u) = z / (1 + exp(-2u)),
+// is the same with another x: one exponential, and no cancellation where tanh nears -1.
+__device__ __forceinline__ float2 silu_exponent(float2 z) { return __fmul2_rn(z, both(-kLog2e)); }
+__device__ __forceinline__ float2 gelu_tanh_exponent(float2 z) {
+  return __fmul2_rn(z, __ffma2_rn(__fmul2_rn(z, z), both(-kLog2e * kGeluA * kGeluB), both(-kLog2e * kGeluA)));
 }
-
-// 0.5 z (1 + tanh(u)) = z sigmoid(2u): one exponential, and no cancellation where tanh nears -1.
-__device__ __forceinline__ float2 gelu_tanh_sigmoid2(float2 z) {
-  const float2 w = __ffma2_rn(__fmul2_rn(z, z), both(-kLog2e * kGeluA * kGeluB), both(-kLog2e * kGeluA));
-  return rcp2(__fadd2_rn(ex2_2(__fmul2_rn(z, w)), both(1.0f)));
-}
+__device__ __forceinline__ float2 logistic2(float2 x) { return rcp2(__fadd2_rn(ex2_2(x), both(1.0f))); }
 
 // The normal distribution's tail q = Phi(-|z|) = erfc(|z| / sqrt 2) / 2 and e = exp(-z^2 / 2), by
 // Hastings' formula (C. Hastings, "Approximations for Digital Computers", 1955, sheet 45; 7.1.26 of
@@ -122,35 +120,62 @@ __device__ __forceinline__ float2 gelu_tanh_sigmoid2(float2 z) {
 // 1.5e-7 for x >= 0.  Halved here.  One reciprocal and one exponential, with e shared by the derivative, where
 // erff takes a branch and some 25 instructions more.  `nz` is -|z| held above -128, where q is 0; for a NaN it is
 // -128, and the NaN comes through e.
+// kN pairs are taken through it step by step, which overlaps their latencies.
+template <int kN>
 struct NormalTail {
-  float2 nz, q, e;
+  float2 nz[kN], q[kN], e[kN];
 };
-__device__ __forceinline__ NormalTail normal_tail2(float2 z) {
-  NormalTail n;
-  n.nz = make_float2(fmaxf(-fabsf(z.x), -128.0f), fmaxf(-fabsf(z.y), -128.0f));
-  const float2 t = rcp2(__ffma2_rn(n.nz, both(-0.3275911f * 0.70710678118654752f), both(1.0f)));
-  float2 p = __ffma2_rn(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
-  p = __ffma2_rn(t, p, both(0.5f * 1.421413741f));
-  p = __ffma2_rn(t, p, both(0.5f * -0.284496736f));
-  p = __ffma2_rn(t, p, both(0.5f * 0.254829592f));
-  n.e = ex2_2(__fmul2_rn(z, __fmul2_rn(z, both(-0.5f * kLog2e))));
-  n.q = __fmul2_rn(__fmul2_rn(t, p), n.e);
+template <int kN>
+__device__ __forceinline__ NormalTail<kN> normal_tail(const float2* z) {
+  NormalTail<kN> n;
+  float2 t[kN], p[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    n.nz[i] = make_float2(fmaxf(-fabsf(z[i].x), -128.0f), fmaxf(-fabsf(z[i].y), -128.0f));
+    t[i] = __ffma2_rn(n.nz[i], both(-0.3275911f * 0.70710678118654752f), both(1.0f));
+  }
+#pragma unroll
+  for (int i = 0; i < kN; ++i) t[i] = rcp2(t[i]);
+#pragma unroll
+  for (int i = 0; i < kN; ++i) n.e[i] = __fmul2_rn(z[i], __fmul2_rn(z[i], both(-0.5f * kLog2e)));
+#pragma unroll
+  for (int i = 0; i < kN; ++i) n.e[i] = ex2_2(n.e[i]);
+#pragma unroll
+  for (int i = 0; i < kN; ++i) p[i] = __ffma2_rn(t[i], both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+#pragma unroll
+  for (int i = 0; i < kN; ++i) p[i] = __ffma2_rn(t[i], p[i], both(0.5f * 1.421413741f));
+#pragma unroll
+  for (int i = 0; i < kN; ++i) p[i] = __ffma2_rn(t[i], p[i], both(0.5f * -0.284496736f));
+#pragma unroll
+  for (int i = 0; i < kN; ++i) p[i] = __ffma2_rn(t[i], p[i], both(0.5f * 0.254829592f));
+#pragma unroll
+  for (int i = 0; i < kN; ++i) n.q[i] = __fmul2_rn(__fmul2_rn(t[i], p[i]), n.e[i]);
   return n;
 }
 
-template <int kAct>
-__device__ __forceinline__ float2 act_value2(float2 z) {
-  if constexpr (kAct == RB_ACT_RELU) return relu2(z);
-  else if constexpr (kAct == RB_ACT_RELU2) {
-    const float2 r = relu2(z);
-    return __fmul2_rn(r, r);
-  } else if constexpr (kAct == RB_ACT_SILU) return __fmul2_rn(z, sigmoid2(z));
-  else if constexpr (kAct == RB_ACT_GELU) {
-    // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
-    const NormalTail n = normal_tail2(z);
-    return __ffma2_rn(n.nz, n.q, make_float2(fmaxf(z.x, 0.0f), fmaxf(z.y, 0.0f)));
-  } else if constexpr (kAct == RB_ACT_GELU_TANH) return __fmul2_rn(z, gelu_tanh_sigmoid2(z));
-  else return z;
+// kN pairs through the activation, in place.
+template <int kAct, int kN>
+__device__ __forceinline__ void act_batch(float2* v) {
+  if constexpr (kAct == RB_ACT_RELU || kAct == RB_ACT_RELU2) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      v[i] = relu2(v[i]);
+      if constexpr (kAct == RB_ACT_RELU2) v[i] = __fmul2_rn(v[i], v[i]);
+    }
+  } else if constexpr (kAct == RB_ACT_GELU) {  // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+    const NormalTail<kN> n = normal_tail<kN>(v);
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      v[i] = __ffma2_rn(n.nz[i], n.q[i], make_float2(fmaxf(v[i].x, 0.0f), fmaxf(v[i].y, 0.0f)));
+  } else if constexpr (kAct == RB_ACT_SILU || kAct == RB_ACT_GELU_TANH) {
+    float2 s[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) s[i] = ex2_2(kAct == RB_ACT_SILU ? silu_exponent(v[i]) : gelu_tanh_exponent(v[i]));
+#pragma unroll
+    for (int i = 0; i < kN; ++i) s[i] = rcp2(__fadd2_rn(s[i], both(1.0f)));
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = __fmul2_rn(v[i], s[i]);
+  }
 }
 
 template <int kAct>
@@ -160,15 +185,15 @@ __device__ __forceinline__ float2 act_derivative2(float2 z) {
   else if constexpr (kAct == RB_ACT_RELU2)
     return make_float2(z.x <= 0.0f ? 0.0f : z.x + z.x, z.y <= 0.0f ? 0.0f : z.y + z.y);
   else if constexpr (kAct == RB_ACT_SILU) {
-    const float2 s = sigmoid2(z);
+    const float2 s = logistic2(silu_exponent(z));
     return __fmul2_rn(s, __ffma2_rn(z, __ffma2_rn(s, both(-1.0f), both(1.0f)), both(1.0f)));
   } else if constexpr (kAct == RB_ACT_GELU) {
-    const NormalTail n = normal_tail2(z);
-    const float2 up = __ffma2_rn(n.q, both(-1.0f), both(1.0f));
-    const float2 phi = make_float2(z.x < 0.0f ? n.q.x : up.x, z.y < 0.0f ? n.q.y : up.y);
-    return __ffma2_rn(__fmul2_rn(z, both(kInvSqrt2Pi)), n.e, phi);
+    const NormalTail<1> n = normal_tail<1>(&z);
+    const float2 up = __ffma2_rn(n.q[0], both(-1.0f), both(1.0f));
+    const float2 phi = make_float2(z.x < 0.0f ? n.q[0].x : up.x, z.y < 0.0f ? n.q[0].y : up.y);
+    return __ffma2_rn(__fmul2_rn(z, both(kInvSqrt2Pi)), n.e[0], phi);
   } else if constexpr (kAct == RB_ACT_GELU_TANH) {
-    const float2 s = gelu_tanh_sigmoid2(z);
+    const float2 s = logistic2(gelu_tanh_exponent(z));
     const float2 t = __fmul2_rn(s, __ffma2_rn(s, both(-1.0f), both(1.0f)));
     const float2 du = __ffma2_rn(__fmul2_rn(z, z), both(3.0f * kGeluA * kGeluB), both(kGeluA));
     const float2 d = __ffma2_rn(__fmul2_rn(z, t), du, s);

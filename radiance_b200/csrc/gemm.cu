@@ -972,7 +972,7 @@ __device__ __forceinline__ void box_add8(float2* v, uint32_t row_addr, int j, ui
 template <int kAct>
 __device__ __forceinline__ void act32(float2 (&v)[16]) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = act_value2<kAct>(v[i]);
+  for (int i = 0; i < 16; i += 8) act_batch<kAct, 8>(v + i);
 }
 
 // 32 accumulator columns of this lane's row (r), columns col0 .. col0 + 31 of the output, at the box's
