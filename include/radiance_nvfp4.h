@@ -427,7 +427,7 @@ int rb_nvfp4_epilogue_backward(const void* grad_y, int64_t ldg, const void* prea
  *   rows[t, j] : the row of pair (t, j): offsets of its expert plus the number of that expert's pairs of
  *                earlier tokens; -1 without a pick;
  *   *loss      : E * sum_e (counts[e] / sum of counts) * (mean over the n routed tokens of p_e), 0 if n = 0;
- *   *routed    : n.
+ *   share[e]   : E * (counts[e] / sum of counts) / n, what rb_nvfp4_route_backward needs of the counts.
  *   logits : tokens x experts of `dtype`, row stride ld;  expert_bias : fp32[experts] or NULL;
  *   valid  : one byte per token or NULL;  weights, picks, rows : tokens x k.
  *   1 <= experts <= 256, 1 <= k <= min(experts, 32), tokens * k + 128 * experts < 2^31.
@@ -437,21 +437,21 @@ int rb_nvfp4_epilogue_backward(const void* grad_y, int64_t ldg, const void* prea
 size_t rb_nvfp4_route_workspace(int64_t tokens, int64_t experts, int k);
 int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
                    const float* expert_bias, const void* valid, int renormalize, float* weights, int32_t* picks,
-                   int32_t* rows, int64_t* counts, int64_t* offsets, float* loss, int32_t* routed, void* workspace,
+                   int32_t* rows, int64_t* counts, int64_t* offsets, float* loss, float* share, void* workspace,
                    size_t workspace_bytes, void* stream);
 
 /*
  * Gradient of rb_nvfp4_route's weights and loss with respect to the logits; the selection and the counts
- * are constants.  With c_e = *grad_loss * E * (counts[e] / sum of counts) / n:
+ * are constants.  With c_e = *grad_loss * share[e]:
  *   grad_logits = p (c - <p, c>) + the picks' part, w (g - <w, g>) at the picks if `renormalize`, else
  *   w g at the picks minus p <w, g>;  rows of tokens that were not routed are 0.
  *   grad_weights (tokens x k) and grad_loss (scalar) may each be NULL; grad_logits has the logits' dtype
  *   and row stride ldo.
  */
 int rb_nvfp4_route_backward(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
-                            int renormalize, const float* weights, const int32_t* picks, const int64_t* counts,
-                            const int32_t* routed, const float* grad_weights, const float* grad_loss,
-                            void* grad_logits, int64_t ldo, void* stream);
+                            int renormalize, const float* weights, const int32_t* picks, const float* share,
+                            const float* grad_weights, const float* grad_loss, void* grad_logits, int64_t ldo,
+                            void* stream);
 
 /*
  * Token rows to the expert-sorted layout: out[rows[t, j]] = x[t] for every pair with a row, and zero in

@@ -105,7 +105,7 @@ SIGNATURES: dict[str, tuple] = {
     "rb_nvfp4_route_backward": (
         _int,
         [_c_void_p, _int, _i64, _i64, _i64, _int, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
-         _c_void_p, _c_void_p, _i64, _c_void_p],
+         _c_void_p, _i64, _c_void_p],
     ),
     "rb_nvfp4_token_dispatch": (
         _int,

@@ -1071,6 +1071,13 @@ __device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, cons
   Tile2 T = tile2_at(cid, g, sm.tile_prefix);
   float2 next_bias = n_my > 0 ? load_bias(T.ncol0 + column_at(0, T.width, 0)) : both(0.0f);
   uint32_t phases = 0;  // bit s: the parity that box s's next residual completes
+  uint32_t coming = 0;  // bit s: a residual is on its way to box s
+  // A wait that ran out ends the epilogue, but not before this warp's own copies have landed (or had the time to).
+  const auto give_up = [&](uint32_t code) {
+    if (lane == 0) record_status(&g_gemm_status, code);
+    for (int s = 0; s < 2; ++s)
+      if ((coming >> s) & 1u) mbar_wait_warp(&bars[s], (phases >> s) & 1u);
+  };
   for (int i = 0; i < n_my; ++i) {
     const int64_t row0 = row_of(T);
     const bool store = row0 < T.row_end;
@@ -1078,18 +1085,18 @@ __device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, cons
     // Frees the boxes and loads the residuals that go into them: of the chunk at `step`, part `part` (and with
     // both boxes for results, of the part or step after it).
     const auto open_boxes = [&](int step, int part) {
-      if (lane != 0) return;
-      bulk_wait_read<0>();
+      if (lane == 0) bulk_wait_read<0>();
       if (!residual || !store) return;
       const int col = T.ncol0 + column_at(i, T.width, step);
+      const bool second = !preact && (kF32 || step + 1 < steps);
+      coming |= second ? 3u : 1u;
+      if (lane != 0) return;
       load_residual(0, row0, col + part * kBoxCols);
-      if (preact) return;
-      if constexpr (kF32) load_residual(1, row0, col + kBoxCols);
-      else if (step + 1 < steps) load_residual(1, row0, T.ncol0 + column_at(i, T.width, step + 1));
+      if (second) load_residual(1, row0, kF32 ? col + kBoxCols : T.ncol0 + column_at(i, T.width, step + 1));
     };
     open_boxes(0, 0);
     if (!__all_sync(0xFFFFFFFFu, mbar_wait_sleep(&sm.acc_full, (uint32_t)(i & 1), 64))) {
-      if (lane == 0) record_status(&g_gemm_status, kStatusTimeoutMma);
+      give_up(kStatusTimeoutMma);
       return;
     }
     tc_fence_after();
@@ -1128,10 +1135,11 @@ __device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, cons
         const int slot = preact ? 0 : kF32 ? part : step;
         if (residual && store) {
           if (!mbar_wait_warp(&bars[slot], (phases >> slot) & 1u)) {
-            if (lane == 0) record_status(&g_gemm_status, kStatusTimeoutTma);
+            give_up(kStatusTimeoutTma);
             return;
           }
           phases ^= 1u << slot;
+          coming &= ~(1u << slot);
         }
         const int box_col = T.ncol0 + col + part * kBoxCols;
         const uint32_t box = boxes + (uint32_t)slot * kOutBox;

@@ -33,7 +33,7 @@ struct RouteArgs {
   int64_t* counts;      // experts
   int64_t* offsets;     // experts + 1
   float* loss;
-  int32_t* routed;      // number of tokens that were routed
+  float* share;         // experts: d loss / d (an expert's probability), of any routed token
   int64_t chunk;        // tokens per block
   int64_t blocks;
   // scratch, per block: pairs of each expert, sums of each expert's probability, routed tokens
@@ -149,7 +149,7 @@ __device__ __forceinline__ void plan_block(const RouteArgs& a, int64_t c0, int64
       a.offsets[x] = offset;
       if (x == a.experts - 1) a.offsets[a.experts] = offset + padded;
     }
-    // loss = E sum_e (count_e / sum of counts) (sum of p_e / n)
+    // loss = sum_e share_e (sum of p_e), share_e = E (count_e / sum of counts) / n
     int32_t n = 0;
     for (int64_t b = x; b < a.blocks; b += kRouteThreads) n += __ldcg(a.nrouted + b);
     n = __reduce_add_sync(0xFFFFFFFFu, n);
@@ -172,9 +172,11 @@ __device__ __forceinline__ void plan_block(const RouteArgs& a, int64_t c0, int64
         pairs += sm.red[w];
         n += sm.n[w];
       }
-      *a.loss = n > 0 ? (float)((double)a.experts * fp / (pairs * (double)n)) : 0.0f;
-      *a.routed = n;
+      sm.red[0] = n > 0 ? (double)a.experts / (pairs * (double)n) : 0.0;
+      *a.loss = (float)(sm.red[0] * fp);
     }
+    __syncthreads();
+    if (x < a.experts) a.share[x] = (float)(sm.red[0] * (double)total);
   }
   __syncthreads();
   for (int64_t ch = c0; ch < c1; ++ch) {
@@ -407,41 +409,27 @@ struct RouteBwdArgs {
   int renormalize;
   const float* weights;
   const int32_t* picks;
-  const int64_t* counts;
-  const int32_t* routed;
+  const float* share;      // experts
   const float* grad_w;     // tokens x k, or nullptr
   const float* grad_loss;  // scalar, or nullptr
   void* grad;              // tokens x experts, row stride ldo
   int64_t ldo;
 };
 
-// dl = p (c - <p, c>) + the picks' part, c_e = grad_loss E f_e / n.  The probabilities are computed
+// dl = p (c - <p, c>) + the picks' part, c_e = grad_loss share_e.  The probabilities are computed
 // again from the logits instead of being stored by the forward pass.
 template <typename T, int LPT, int ITEMS>
 __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const RouteBwdArgs a) {
   constexpr int kGroups = kRouteThreads / LPT;
-  __shared__ float csm[kMaxExperts];
-  __shared__ float pairs_sm[kRouteWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
   const int gl = lane & (LPT - 1), gid = threadIdx.x / LPT;
-  {
-    const int64_t cnt = (int)threadIdx.x < a.experts ? a.counts[threadIdx.x] : 0;
-    float pairs = (float)cnt;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) pairs += __shfl_xor_sync(0xFFFFFFFFu, pairs, o);
-    if (lane == 0) pairs_sm[warp] = pairs;
-    __syncthreads();
-    pairs = 0.0f;
-    for (int w = 0; w < kRouteWarps; ++w) pairs += pairs_sm[w];
-    const float n = (float)*a.routed;
-    const float g = a.grad_loss != nullptr && n > 0.0f ? *a.grad_loss : 0.0f;
-    if ((int)threadIdx.x < a.experts)
-      csm[threadIdx.x] = g != 0.0f ? g * (float)a.experts * ((float)cnt / pairs) / n : 0.0f;
-    __syncthreads();
-  }
+  const float g = a.grad_loss != nullptr ? *a.grad_loss : 0.0f;
   float c[ITEMS];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) c[i] = i * LPT + gl < a.experts ? csm[i * LPT + gl] : 0.0f;
+  for (int i = 0; i < ITEMS; ++i) {
+    const int e = i * LPT + gl;
+    c[i] = e < a.experts && g != 0.0f ? g * a.share[e] : 0.0f;
+  }
   for (int64_t tb = (int64_t)blockIdx.x * kGroups; tb < a.tokens; tb += (int64_t)gridDim.x * kGroups) {
     const int64_t t = tb + gid;
     const bool in_t = t < a.tokens;
@@ -960,11 +948,11 @@ size_t rb_nvfp4_route_workspace(int64_t tokens, int64_t experts, int k) {
 
 int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
                    const float* expert_bias, const void* valid, int renormalize, float* weights, int32_t* picks,
-                   int32_t* rows, int64_t* counts, int64_t* offsets, float* loss, int32_t* routed, void* workspace,
+                   int32_t* rows, int64_t* counts, int64_t* offsets, float* loss, float* share, void* workspace,
                    size_t workspace_bytes, void* stream) {
   const char* what = "nvfp4 route";
   if (const int rc = check_route(what, dtype, tokens, experts, ld, k)) return rc;
-  if (counts == nullptr || offsets == nullptr || loss == nullptr || routed == nullptr || workspace == nullptr ||
+  if (counts == nullptr || offsets == nullptr || loss == nullptr || share == nullptr || workspace == nullptr ||
       (tokens > 0 && (logits == nullptr || weights == nullptr || picks == nullptr || rows == nullptr)) ||
       unaligned(counts, 8) || unaligned(offsets, 8) || unaligned(workspace, 4))
     return route_failed(RB_ERR_ARG, "%s: null or misaligned pointer argument", what);
@@ -986,7 +974,7 @@ int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t expert
   a.counts = counts;
   a.offsets = offsets;
   a.loss = loss;
-  a.routed = routed;
+  a.share = share;
   a.chunk = route_chunk(tokens, a.experts, k);
   a.blocks = tokens > 0 ? (tokens + a.chunk - 1) / a.chunk : 1;
   a.psum = reinterpret_cast<float*>(workspace);
@@ -1010,15 +998,15 @@ int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t expert
 }
 
 int rb_nvfp4_route_backward(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
-                            int renormalize, const float* weights, const int32_t* picks, const int64_t* counts,
-                            const int32_t* routed, const float* grad_weights, const float* grad_loss,
-                            void* grad_logits, int64_t ldo, void* stream) {
+                            int renormalize, const float* weights, const int32_t* picks, const float* share,
+                            const float* grad_weights, const float* grad_loss, void* grad_logits, int64_t ldo,
+                            void* stream) {
   const char* what = "nvfp4 route_backward";
   if (const int rc = check_route(what, dtype, tokens, experts, ld, k)) return rc;
   if (ldo < experts) return route_failed(RB_ERR_SHAPE, "%s: the gradient's row stride %lld is below %lld experts", what, ldo, experts);
   if (tokens == 0) return RB_OK;
-  if (logits == nullptr || weights == nullptr || picks == nullptr || counts == nullptr || routed == nullptr ||
-      grad_logits == nullptr || unaligned(counts, 8))
+  if (logits == nullptr || weights == nullptr || picks == nullptr || share == nullptr ||
+      grad_logits == nullptr)
     return route_failed(RB_ERR_ARG, "%s: null or misaligned pointer argument", what);
   if (!route_device(what)) return RB_ERR_DEVICE;
   rb::RouteBwdArgs a = {};
@@ -1030,8 +1018,7 @@ int rb_nvfp4_route_backward(const void* logits, int dtype, int64_t tokens, int64
   a.renormalize = renormalize;
   a.weights = weights;
   a.picks = picks;
-  a.counts = counts;
-  a.routed = routed;
+  a.share = share;
   a.grad_w = grad_weights;
   a.grad_loss = grad_loss;
   a.grad = grad_logits;

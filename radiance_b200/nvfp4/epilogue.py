@@ -45,6 +45,14 @@ def _call(what: str, device: torch.device, fn, *args) -> None:
         _lib.check(rc, what)
 
 
+def _size(device: torch.device, fn, *args) -> int:
+    """A workspace size, asked with ``device`` current (it goes by the device's SMs and its budget)."""
+    if device.index == torch.cuda.current_device():
+        return int(fn(*args))
+    with torch.cuda.device(device):
+        return int(fn(*args))
+
+
 def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """A 2-D tensor whose rows are contiguous and do not overlap, and its row stride in elements."""
     r, c = x.shape
@@ -177,6 +185,10 @@ def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     return lda != ldb or at < width or at + width > lda
 
 
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
+
+
 def _operand(q: NVFP4Tensor, device: torch.device, what: str) -> None:
     """Refuses an operand whose tensors the kernel would read past or cannot read."""
     rows, k2 = q.packed.shape
@@ -235,8 +247,7 @@ def epilogue_mm(a: NVFP4Tensor, b: NVFP4Tensor, *, bias: torch.Tensor | None = N
         _like("out", out, (m, n), out_dtype, dev, what)
         if _tma_rows(out) is not out:
             raise ValueError(f"{what}: out must be 16-byte aligned with contiguous rows and 16-byte row strides")
-        if residual is not None and _share_memory(out, _rows(residual)[0]) and not (
-                out.data_ptr() == residual.data_ptr() and out.stride() == residual.stride()):
+        if residual is not None and _share_memory(out, _rows(residual)[0]) and not _same(out, residual):
             raise ValueError(f"{what}: out overlaps the residual without being the residual")
         ldo = _rows(out)[1]
     if residual is not None:
@@ -290,10 +301,13 @@ def epilogue_backward(grad_y: torch.Tensor, preact: torch.Tensor | None = None, 
         if _rows(out)[0] is not out:
             raise ValueError(f"{what}: out must have contiguous rows")
         ldo = _rows(out)[1]
+        for name, t in (("gradient", grad_y), ("pre-activations", z)):
+            if t is not None and _share_memory(out, t) and not _same(out, t):
+                raise ValueError(f"{what}: out overlaps the {name} without being the same tensor")
     gs = torch.empty((), dtype=torch.float32, device=dev)
     sums = torch.empty(cols, dtype=torch.float32, device=dev) if bias_grad else None
     lib = _lib.load()
-    need = int(lib.rb_nvfp4_epilogue_backward_workspace(rows, cols))
+    need = _size(dev, lib.rb_nvfp4_epilogue_backward_workspace, rows, cols)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     tok = _trace.begin("epilogue", rows * cols * grad_y.element_size() * (2 + (z is not None)))
     _call(what, dev, lib.rb_nvfp4_epilogue_backward, grad_y.data_ptr(), ldg, None if z is None else z.data_ptr(), ldz,

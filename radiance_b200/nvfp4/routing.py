@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import _trace
-from .epilogue import _call, _dtype_of, _like, _rows
+from .epilogue import _call, _dtype_of, _like, _rows, _size
 from .quantize import _require_cuda
 
 MAX_EXPERTS = 256  # the grouped GEMM's group limit
@@ -50,30 +50,33 @@ def _route(logits, k, expert_bias, valid, renormalize):
     tokens, experts = logits.shape
     dev = logits.device
     weights = torch.empty(tokens, k, dtype=torch.float32, device=dev)
-    picks, rows = torch.empty(2, tokens, k, dtype=torch.int32, device=dev).unbind(0)
-    whole = torch.empty(2 * experts + 1, dtype=torch.int64, device=dev)
-    counts, offsets = whole[:experts], whole[experts:]
+    # Tensors of their own: what a caller does to one in place (an all-reduce of the counts) leaves the others'
+    # versions alone, and the backward reads `share`, which no caller sees, instead of the counts.
+    picks = torch.empty(tokens, k, dtype=torch.int32, device=dev)
+    rows = torch.empty(tokens, k, dtype=torch.int32, device=dev)
+    counts = torch.empty(experts, dtype=torch.int64, device=dev)
+    offsets = torch.empty(experts + 1, dtype=torch.int64, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    routed = torch.empty((), dtype=torch.int32, device=dev)
+    share = torch.empty(experts, dtype=torch.float32, device=dev)
     lib = _lib.load()
-    need = int(lib.rb_nvfp4_route_workspace(tokens, experts, k))
-    ws = torch.empty(max(need, 4), dtype=torch.uint8, device=dev)
+    need = _size(dev, lib.rb_nvfp4_route_workspace, tokens, experts, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
     tok = _trace.begin("route", logits.numel() * logits.element_size() + 12 * tokens * k)
     _call(what, dev, lib.rb_nvfp4_route, logits.data_ptr(), code, tokens, experts, ld, k,
           None if expert_bias is None else expert_bias.data_ptr(), None if valid is None else valid.data_ptr(),
           int(renormalize), weights.data_ptr(), picks.data_ptr(), rows.data_ptr(), counts.data_ptr(),
-          offsets.data_ptr(), loss.data_ptr(), routed.data_ptr(), ws.data_ptr(), need)
+          offsets.data_ptr(), loss.data_ptr(), share.data_ptr(), ws.data_ptr(), need)
     _trace.end(tok)
-    return weights, loss, picks, counts, offsets, rows, routed
+    return weights, loss, picks, counts, offsets, rows, share
 
 
 class _RouteFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, expert_bias, valid, renormalize):
         ctx.set_materialize_grads(False)
-        weights, loss, picks, counts, offsets, rows, routed = _route(logits, k, expert_bias, valid, renormalize)
+        weights, loss, picks, counts, offsets, rows, share = _route(logits, k, expert_bias, valid, renormalize)
         ctx.mark_non_differentiable(picks, counts, offsets, rows)
-        ctx.save_for_backward(logits, weights, picks, counts, routed)
+        ctx.save_for_backward(logits, weights, picks, share)
         ctx.renormalize = renormalize
         return weights, loss, picks, counts, offsets, rows
 
@@ -83,7 +86,7 @@ class _RouteFn(torch.autograd.Function):
         if grad_w is None and grad_loss is None:
             return None, None, None, None, None
         what = "nvfp4.route backward"
-        logits, weights, picks, counts, routed = ctx.saved_tensors
+        logits, weights, picks, share = ctx.saved_tensors
         tokens, experts = logits.shape
         grad = torch.empty(tokens, experts, dtype=logits.dtype, device=logits.device)
         x, ld = _rows(logits)
@@ -91,9 +94,9 @@ class _RouteFn(torch.autograd.Function):
             grad_w = grad_w.contiguous()
         tok = _trace.begin("route", 2 * x.numel() * x.element_size() + 12 * picks.numel())
         _call(what, x.device, _lib.load().rb_nvfp4_route_backward, x.data_ptr(), _dtype_of(x, what), tokens, experts,
-              ld, picks.shape[1], int(ctx.renormalize), weights.data_ptr(), picks.data_ptr(), counts.data_ptr(),
-              routed.data_ptr(), None if grad_w is None else grad_w.data_ptr(),
-              None if grad_loss is None else grad_loss.data_ptr(), grad.data_ptr(), experts)
+              ld, picks.shape[1], int(ctx.renormalize), weights.data_ptr(), picks.data_ptr(), share.data_ptr(),
+              None if grad_w is None else grad_w.data_ptr(), None if grad_loss is None else grad_loss.data_ptr(),
+              grad.data_ptr(), experts)
         _trace.end(tok)
         return grad, None, None, None, None
 

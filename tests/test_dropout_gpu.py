@@ -162,6 +162,30 @@ def test_stream_and_graph(nv):
         assert torch.equal(out, want[s])
 
 
+def test_fresh_seeds_in_a_graph(nv):
+    """Without a seed every replay draws another mask, and its backward the same one again."""
+    x = torch.ones(4096, device="cuda", requires_grad=True)
+    gy = torch.ones(4096, device="cuda")
+    torch.autograd.grad(nv.dropout(x, 0.5), x, gy)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = nv.dropout(x, 0.5)
+        (gx,) = torch.autograd.grad(y, x, gy)
+    seen = []
+    for _ in range(3):
+        g.replay()
+        assert torch.equal(gx, y) and 0.4 < (y > 0).float().mean().item() < 0.6  # x = gy = 1
+        seen.append(y.detach().clone())
+    assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
+def test_second_order_is_refused(nv):
+    x = _rand(64).requires_grad_()
+    (g,) = torch.autograd.grad(nv.dropout(x, 0.5, seed=1).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
 # ------------------------------------------------------------------------------------------------
 # epilogue_backward
 # ------------------------------------------------------------------------------------------------
@@ -278,5 +302,10 @@ def test_refusals(nv):
         nv.epilogue_backward(x, dropout_p=0.5)
     with pytest.raises(ValueError, match="non-empty"):
         nv.epilogue_backward(x[:0])
+    buf = torch.zeros(9, 16, device="cuda")
+    with pytest.raises(ValueError, match="overlaps the gradient"):
+        nv.epilogue_backward(buf[:8], out=buf[1:])
+    with pytest.raises(ValueError, match="overlaps the pre-activations"):
+        nv.epilogue_backward(x, buf[1:], activation="silu", out=buf[:8])
     with pytest.raises(ValueError, match="out must have contiguous rows"):
         nv.epilogue_backward(x, out=torch.empty(16, 8, device="cuda").t())

@@ -98,8 +98,8 @@ def test_entry_points_refuse_on_the_host():
                dict(ld=7), dict(tokens=-1), dict(tokens=1 << 31)):
         assert route(**kw) == 1, kw
     assert route(logits=None) == 2 and route(ws=None) == 2 and route(counts=ctypes.c_void_p(4)) == 2
-    assert lib.rb_nvfp4_route_backward(buf, 1, 4, 8, 8, 2, 1, buf, buf, buf, buf, None, None, buf, 7, None) == 1
-    assert lib.rb_nvfp4_route_backward(buf, 1, 4, 8, 8, 2, 1, None, buf, buf, buf, None, None, buf, 8, None) == 2
+    assert lib.rb_nvfp4_route_backward(buf, 1, 4, 8, 8, 2, 1, buf, buf, buf, None, None, buf, 7, None) == 1
+    assert lib.rb_nvfp4_route_backward(buf, 1, 4, 8, 8, 2, 1, None, buf, buf, None, None, buf, 8, None) == 2
 
     def disp(dtype=0, tokens=4, d=8, ld=8, k=2, e=4, n=512, ldo=8, out=buf):
         return lib.rb_nvfp4_token_dispatch(buf, dtype, tokens, d, ld, buf, k, buf, buf, e, out, n, ldo, None)

@@ -223,6 +223,23 @@ def test_linear_gradients(nv, act, p, has_res, bias, dtype):
         assert torch.equal(got[-1], gy)
 
 
+@pytest.mark.parametrize("recipe", [dict(save_activations=False), dict(grad_gemms=False),
+                                    dict(stochastic_rounding=False, hadamard=False)])
+def test_linear_recipes(nv, recipe):
+    """Every recipe's backward takes the epilogue's gradient as it takes the plain layer's."""
+    torch.manual_seed(1)
+    layer = nv.FP4Linear(256, 384, recipe=nv.FP4Recipe(**recipe)).cuda()
+    layer.refresh_fp4_cache()
+    x = _rand(128, 256, dtype=torch.bfloat16, seed=1).requires_grad_()
+    res, gy = _rand(128, 384, dtype=torch.bfloat16, seed=2), _rand(128, 384, dtype=torch.bfloat16, seed=3, std=1e-2)
+    y = layer(x, activation="silu", dropout_p=0.1, dropout_seed=7, residual=res)
+    got = torch.autograd.grad(y, (x, layer.weight), gy)
+    z = layer(x)
+    gz, _, _ = nv.epilogue_backward(gy, z.detach(), activation="silu", dropout_p=0.1, seed=7)
+    ref = torch.autograd.grad(z, (x, layer.weight), gz)
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
 def test_linear_fallback_and_refusals(nv):
     torch.manual_seed(1)
     layer = nv.FP4Linear(256, 384).cuda()

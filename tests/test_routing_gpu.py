@@ -173,6 +173,16 @@ def test_only_one_gradient(nv):
     assert a.abs().max() > 0 and b.abs().max() > 0
 
 
+def test_counts_may_be_reduced_in_place(nv):
+    """A data-parallel job adds up the counts of its ranks before the backward pass."""
+    logits = _rand(100, 9, seed=1).requires_grad_()
+    want = torch.autograd.grad(nv.route(logits, 2).balance_loss, logits)[0]
+    r = nv.route(logits, 2)
+    r.counts.mul_(4)
+    r.rows.add_(1)
+    assert torch.equal(torch.autograd.grad(r.balance_loss, logits)[0], want)
+
+
 def test_route_gradient_against_differences(nv):
     """Central differences of the fp32 forward, with the selection unchanged by the step."""
     logits = _rand(16, 6, seed=4).requires_grad_()

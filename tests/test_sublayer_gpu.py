@@ -149,6 +149,20 @@ def test_block_in_a_graph(nv):
         assert torch.equal(a, b)
 
 
+def test_a_batch_of_padding(nv):
+    """No token takes part: the output is the residual, every gradient of the experts and the logits is zero."""
+    ex = _experts(nv)
+    x = _rand(130, 256, seed=1).requires_grad_()
+    logits = torch.full((130, 6), float("nan"), device="cuda", requires_grad=True)
+    y, r = ex.forward_routed(x, logits, 2, valid=torch.zeros(130, dtype=torch.bool, device="cuda"), residual=x)
+    assert torch.equal(y, x) and r.balance_loss == 0 and (r.counts == 0).all()
+    gy = _rand(130, 256, seed=2)
+    ((y * gy).float().sum() + r.balance_loss).backward()
+    assert torch.equal(x.grad, gy) and (logits.grad == 0).all()
+    for name, p in ex.named_parameters():
+        assert (p.grad == 0).all(), name
+
+
 def test_routed_experts_without_tokens(nv):
     ex = _experts(nv)
     y, r = ex.forward_routed(torch.empty(0, 256, device="cuda", dtype=torch.bfloat16),
