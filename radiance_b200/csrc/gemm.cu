@@ -1095,6 +1095,7 @@ __device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, cons
       if (second) load_residual(1, row0, kF32 ? col + kBoxCols : T.ncol0 + column_at(i, T.width, step + 1));
     };
     open_boxes(0, 0);
+    const Tile2 Tn = i + 1 < n_my ? tile2_at(cid + (i + 1) * ncl, g, sm.tile_prefix) : T;
     if (!__all_sync(0xFFFFFFFFu, mbar_wait_sleep(&sm.acc_full, (uint32_t)(i & 1), 64))) {
       give_up(kStatusTimeoutMma);
       return;
@@ -1120,12 +1121,8 @@ __device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, cons
       if (step == 0 && mine_sc) tc_fence_before();
       __syncwarp();
       if (step == 0 && mine_sc && lane == 0) release();
-      if (step + 1 < steps) {
-        next_bias = load_bias(T.ncol0 + column_at(i, T.width, step + 1));
-      } else if (i + 1 < n_my) {
-        const Tile2 Tn = tile2_at(cid + (i + 1) * ncl, g, sm.tile_prefix);
-        next_bias = load_bias(Tn.ncol0 + column_at(i + 1, Tn.width, 0));
-      }
+      if (step + 1 < steps) next_bias = load_bias(T.ncol0 + column_at(i, T.width, step + 1));
+      else if (i + 1 < n_my) next_bias = load_bias(Tn.ncol0 + column_at(i + 1, Tn.width, 0));
 #pragma unroll
       for (int part = 0; part < kParts; ++part) {
         if (part > 0 && preact) {
@@ -1161,7 +1158,7 @@ __device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, cons
         }
       }
     }
-    T = tile2_at(min(cid + (i + 1) * ncl, g.n_tiles - 1), g, sm.tile_prefix);
+    T = Tn;
   }
 }
 
