@@ -1022,6 +1022,28 @@ __device__ __forceinline__ void fused_columns(const uint32_t* r, float alpha, co
   for (int j = 0; j < 4; ++j) box_store8<kF32>(v + 4 * j, row_addr, j0 + j, sw);
 }
 
+// tcgen05.wait::ld for the 64 registers of two x32 loads, with the registers as operands: nothing that reads
+// them can be scheduled above the wait.
+#define RB_TMEM_WAIT_X64(r)                                                                                    \
+  do {                                                                                                        \
+    asm volatile("tcgen05.wait::ld.sync.aligned;"                                                             \
+                 :"+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),  \
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),  \
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),  \
+                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),  \
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),  \
+                 "+r"(r[31]) \
+                 ::"memory");                                                                                 \
+    asm volatile(""                                                                                           \
+                 :"+r"(r[32]), "+r"(r[33]), "+r"(r[34]), "+r"(r[35]), "+r"(r[36]), "+r"(r[37]),  \
+                 "+r"(r[38]), "+r"(r[39]), "+r"(r[40]), "+r"(r[41]), "+r"(r[42]), "+r"(r[43]),  \
+                 "+r"(r[44]), "+r"(r[45]), "+r"(r[46]), "+r"(r[47]), "+r"(r[48]), "+r"(r[49]),  \
+                 "+r"(r[50]), "+r"(r[51]), "+r"(r[52]), "+r"(r[53]), "+r"(r[54]), "+r"(r[55]),  \
+                 "+r"(r[56]), "+r"(r[57]), "+r"(r[58]), "+r"(r[59]), "+r"(r[60]), "+r"(r[61]),  \
+                 "+r"(r[62]), "+r"(r[63]) \
+                 ::"memory");                                                                                 \
+  } while (0)
+
 // One epilogue warp of the two-SM kernel in fused mode: the TMEM lanes of its warp id mod 4, and every other
 // 64-column chunk of the tile.  It stages its results in boxes of 32 rows x 128 bytes: a chunk is one box of
 // bf16 or two of fp32.  The residual of a box is loaded by TMA into the box that its result is staged in,
@@ -1117,7 +1139,7 @@ __device__ __forceinline__ void fused_epilogue(Smem& sm, const GemmArgs& g, cons
       RB_TMEM_LD_X32(taddr + 32, (r + 32));
       if (g.bias != nullptr) reinterpret_cast<float2*>(bias_sm)[lane] = next_bias;
       if (step > 0 && (kF32 || preact)) open_boxes(step, 0);
-      tmem_ld_wait();
+      RB_TMEM_WAIT_X64(r);
       if (step == 0 && mine_sc) tc_fence_before();
       __syncwarp();
       if (step == 0 && mine_sc && lane == 0) release();
