@@ -166,6 +166,8 @@ int num_sms(int device);
 int sm_budget(int device);
 int set_sm_budget(int device, int sms);
 int current_device();
+// Whether `device` is an sm_100 GPU (asked once per device); sets the error text for `what` if not.
+bool sm100(int device, const char* what);
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no link-time libcuda).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();

@@ -240,12 +240,7 @@ namespace {
 
 bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
-bool on_sm100(const char* what) {
-  int major = 0;
-  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, rb_host::current_device());
-  if (major != 10) rb_host::set_error("%s: the current device is not an sm_100 GPU", what);
-  return major == 10;
-}
+bool on_sm100(const char* what) { return rb_host::sm100(rb_host::current_device(), what); }
 
 int launched(const char* what) {
   const cudaError_t e = cudaGetLastError();

@@ -24,6 +24,17 @@ int current_device() {
   return dev;
 }
 
+bool sm100(int device, const char* what) {
+  static int major[64] = {0};
+  int m = device >= 0 && device < 64 ? major[device] : 0;
+  if (m == 0) {
+    cudaDeviceGetAttribute(&m, cudaDevAttrComputeCapabilityMajor, device);
+    if (device >= 0 && device < 64) major[device] = m;
+  }
+  if (m != 10) set_error("%s: the current device is not an sm_100 GPU", what);
+  return m == 10;
+}
+
 int num_sms(int device) {
   static int cache[64] = {0};
   if (device < 0 || device >= 64) return 148;

@@ -815,12 +815,7 @@ int route_failed(int code, const char* fmt, const char* what, long long x = 0, l
   return code;
 }
 
-bool route_device(const char* what) {
-  int major = 0;
-  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, rb_host::current_device());
-  if (major != 10) rb_host::set_error("%s: the current device is not an sm_100 GPU", what);
-  return major == 10;
-}
+bool route_device(const char* what) { return rb_host::sm100(rb_host::current_device(), what); }
 
 int route_launched(const char* what) {
   const cudaError_t e = cudaGetLastError();

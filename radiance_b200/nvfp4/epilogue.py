@@ -45,6 +45,17 @@ def _call(what: str, device: torch.device, fn, *args) -> None:
         _lib.check(rc, what)
 
 
+def _first_order(backward):
+    """``once_differentiable`` for a Function's backward, entered only where it matters: outside
+    ``create_graph`` grad mode is off already, and its bookkeeping costs as much as a launch."""
+    checked = once_differentiable(backward)
+
+    def wrapper(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return wrapper
+
+
 def _size(device: torch.device, fn, *args) -> int:
     """A workspace size, asked with ``device`` current (it goes by the device's SMs and its budget)."""
     if device.index == torch.cuda.current_device():
@@ -56,6 +67,8 @@ def _size(device: torch.device, fn, *args) -> int:
 def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """A 2-D tensor whose rows are contiguous and do not overlap, and its row stride in elements."""
     r, c = x.shape
+    if x.is_contiguous():
+        return x, c
     if (c > 1 and x.stride(1) != 1) or (r > 1 and x.stride(0) < c):
         x = x.contiguous()
     return x, (x.stride(0) if r > 1 else c)
@@ -120,7 +133,7 @@ class _DropoutFn(torch.autograd.Function):
         return _dropout(x, residual, p, seed)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad):
         (seed,) = ctx.saved_tensors
         gx = None

@@ -14,11 +14,10 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import _trace
-from .epilogue import _call, _dtype_of, _like, _rows, _size
+from .epilogue import _call, _dtype_of, _first_order, _like, _rows, _size
 from .quantize import _require_cuda
 
 MAX_EXPERTS = 256  # the grouped GEMM's group limit
@@ -81,7 +80,7 @@ class _RouteFn(torch.autograd.Function):
         return weights, loss, picks, counts, offsets, rows
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad_w, grad_loss, *_):
         if grad_w is None and grad_loss is None:
             return None, None, None, None, None
@@ -143,17 +142,17 @@ def route(logits: torch.Tensor, k: int, *, expert_bias: torch.Tensor | None = No
 # ------------------------------------------------------------------------------------------------
 
 
-def _plan(r: Routing, device: torch.device, what: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, int]:
-    """(rows, counts, offsets, number of experts) of a routing, checked."""
+def _plan(r: Routing, device: torch.device, what: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(rows, counts, offsets) of a routing, checked."""
     rows, counts, offsets = r.rows, r.counts, r.offsets
-    if rows.dim() != 2 or rows.dtype != torch.int32 or counts.dtype != torch.int64 or offsets.dtype != torch.int64 \
-            or offsets.shape != (counts.numel() + 1,) or counts.dim() != 1:
+    if rows.dtype != torch.int32 or counts.dtype != torch.int64 or offsets.dtype != torch.int64 or rows.dim() != 2 \
+            or counts.dim() != 1 or offsets.shape != (counts.shape[0] + 1,):
         raise ValueError(f"{what}: the routing needs int32 rows (tokens, k) and int64 counts (E,) and offsets (E + 1,)")
     if rows.device != device or counts.device != device or offsets.device != device:
         raise ValueError(f"{what}: the routing is on {rows.device}, the rows on {device}")
     if rows.shape[1] < 1 or r.num_rows < 0:
         raise ValueError(f"{what}: the routing needs at least one pick per token and num_rows >= 0")
-    return rows.contiguous(), counts.contiguous(), offsets.contiguous(), counts.numel()
+    return rows.contiguous(), counts.contiguous(), offsets.contiguous()
 
 
 def _dispatch(x, rows, counts, offsets, num_rows):
@@ -209,7 +208,7 @@ class _DispatchFn(torch.autograd.Function):
         return _dispatch(x, rows, counts, offsets, num_rows)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad):
         (rows,) = ctx.saved_tensors
         return _combine(grad, rows, None, None), None, None, None, None
@@ -222,7 +221,7 @@ class _CombineFn(torch.autograd.Function):
         return _combine(y, rows, weights, residual)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad):
         y, weights, rows, counts, offsets = ctx.saved_tensors
         gy = gw = None
@@ -238,7 +237,7 @@ def token_dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     what = "nvfp4.token_dispatch"
     _require_cuda(x, what)
     _dtype_of(x, what)
-    rows, counts, offsets, _ = _plan(routing, x.device, what)
+    rows, counts, offsets = _plan(routing, x.device, what)
     if x.dim() != 2 or x.shape[0] != rows.shape[0] or x.shape[1] < 1:
         raise ValueError(f"{what}: rows of shape ({rows.shape[0]}, d) expected, got {tuple(x.shape)}")
     if torch.is_grad_enabled() and x.requires_grad:
@@ -254,7 +253,7 @@ def token_combine(y: torch.Tensor, routing: Routing, *, residual: torch.Tensor |
     what = "nvfp4.token_combine"
     _require_cuda(y, what)
     _dtype_of(y, what)
-    rows, counts, offsets, _ = _plan(routing, y.device, what)
+    rows, counts, offsets = _plan(routing, y.device, what)
     tokens, k = rows.shape
     if y.dim() != 2 or y.shape[0] != routing.num_rows or y.shape[1] < 1:
         raise ValueError(f"{what}: expert rows of shape ({routing.num_rows}, d) expected, got {tuple(y.shape)}")
