@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define RB_NVFP4_ABI_VERSION 8
+#define RB_NVFP4_ABI_VERSION 9
 
 /* Input element types. */
 #define RB_DTYPE_BF16 0
@@ -439,6 +439,17 @@ int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t expert
                    const float* expert_bias, const void* valid, int renormalize, float* weights, int32_t* picks,
                    int32_t* rows, int64_t* counts, int64_t* offsets, float* loss, float* share, void* workspace,
                    size_t workspace_bytes, void* stream);
+
+/*
+ * rb_nvfp4_route with the counts written a second time, to plan_counts (8-byte aligned, or NULL).  The row moves
+ * below zero the rows between counts[e] and the end of expert e's group, so the counts they are given must stay
+ * what the routing wrote: a caller whose counts are changed in place meanwhile (added up over the ranks of
+ * a data-parallel job) passes them plan_counts.
+ */
+int rb_nvfp4_route_plan(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
+                        const float* expert_bias, const void* valid, int renormalize, float* weights, int32_t* picks,
+                        int32_t* rows, int64_t* counts, int64_t* plan_counts, int64_t* offsets, float* loss,
+                        float* share, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Gradient of rb_nvfp4_route's weights and loss with respect to the logits; the selection and the counts

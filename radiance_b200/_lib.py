@@ -102,6 +102,11 @@ SIGNATURES: dict[str, tuple] = {
         [_c_void_p, _int, _i64, _i64, _i64, _int, _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p,
          _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p],
     ),
+    "rb_nvfp4_route_plan": (
+        _int,
+        [_c_void_p, _int, _i64, _i64, _i64, _int, _c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, ctypes.c_size_t, _c_void_p],
+    ),
     "rb_nvfp4_route_backward": (
         _int,
         [_c_void_p, _int, _i64, _i64, _i64, _int, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
@@ -132,7 +137,7 @@ SIGNATURES: dict[str, tuple] = {
 
 RB_PEER_HANDLE_BYTES = 64
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 RB_DTYPE_BF16 = 0
 RB_DTYPE_F32 = 1

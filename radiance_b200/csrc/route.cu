@@ -31,6 +31,7 @@ struct RouteArgs {
   int32_t* picks;       // tokens x k, -1: none
   int32_t* rows;        // tokens x k
   int64_t* counts;      // experts
+  int64_t* plan_counts; // the same again, or nullptr
   int64_t* offsets;     // experts + 1
   float* loss;
   float* share;         // experts: d loss / d (an expert's probability), of any routed token
@@ -146,6 +147,7 @@ __device__ __forceinline__ void plan_block(const RouteArgs& a, int64_t c0, int64
   if (summary) {
     if (x < a.experts) {
       a.counts[x] = total;
+      if (a.plan_counts != nullptr) a.plan_counts[x] = total;
       a.offsets[x] = offset;
       if (x == a.experts - 1) a.offsets[a.experts] = offset + padded;
     }
@@ -941,15 +943,15 @@ size_t rb_nvfp4_route_workspace(int64_t tokens, int64_t experts, int k) {
   return (size_t)(blocks * (6 * experts + 4));
 }
 
-int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
-                   const float* expert_bias, const void* valid, int renormalize, float* weights, int32_t* picks,
-                   int32_t* rows, int64_t* counts, int64_t* offsets, float* loss, float* share, void* workspace,
-                   size_t workspace_bytes, void* stream) {
+int rb_nvfp4_route_plan(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
+                        const float* expert_bias, const void* valid, int renormalize, float* weights, int32_t* picks,
+                        int32_t* rows, int64_t* counts, int64_t* plan_counts, int64_t* offsets, float* loss,
+                        float* share, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "nvfp4 route";
   if (const int rc = check_route(what, dtype, tokens, experts, ld, k)) return rc;
   if (counts == nullptr || offsets == nullptr || loss == nullptr || share == nullptr || workspace == nullptr ||
       (tokens > 0 && (logits == nullptr || weights == nullptr || picks == nullptr || rows == nullptr)) ||
-      unaligned(counts, 8) || unaligned(offsets, 8) || unaligned(workspace, 4))
+      unaligned(counts, 8) || unaligned(plan_counts, 8) || unaligned(offsets, 8) || unaligned(workspace, 4))
     return route_failed(RB_ERR_ARG, "%s: null or misaligned pointer argument", what);
   if (!route_device(what)) return RB_ERR_DEVICE;
   if (workspace_bytes < rb_nvfp4_route_workspace(tokens, experts, k))
@@ -967,6 +969,7 @@ int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t expert
   a.picks = picks;
   a.rows = rows;
   a.counts = counts;
+  a.plan_counts = plan_counts;
   a.offsets = offsets;
   a.loss = loss;
   a.share = share;
@@ -990,6 +993,14 @@ int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t expert
     rb::route_plan_kernel<<<workers + 1, rb::kRouteThreads, 0, st>>>(a);
   }
   return route_launched(what);
+}
+
+int rb_nvfp4_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
+                   const float* expert_bias, const void* valid, int renormalize, float* weights, int32_t* picks,
+                   int32_t* rows, int64_t* counts, int64_t* offsets, float* loss, float* share, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  return rb_nvfp4_route_plan(logits, dtype, tokens, experts, ld, k, expert_bias, valid, renormalize, weights, picks,
+                             rows, counts, nullptr, offsets, loss, share, workspace, workspace_bytes, stream);
 }
 
 int rb_nvfp4_route_backward(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,

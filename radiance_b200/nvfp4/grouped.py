@@ -460,7 +460,7 @@ class FP4BatchedExperts(nn.Module):
         # all rows, so both are cut to 0 there.
         start = routing.offsets[:-1]
         row = torch.arange(routing.num_rows, device=x.device).unsqueeze(1)
-        hot = ((row >= start) & (row < start + routing.counts)).to(xs.dtype)
+        hot = ((row >= start) & (row < start + routing.plan_counts)).to(xs.dtype)
         h = torch.addmm(self.gate_up(xs, routing.offsets), hot, self.gate_up_b.squeeze(1).to(xs.dtype))
         h = torch.where(row < routing.offsets[-1], h, 0)
         y = self.down(swiglu(h, "split"), routing.offsets)

@@ -34,6 +34,9 @@ class Routing(NamedTuple):
     offsets: torch.Tensor  # (experts + 1,) int64: first row of each expert's group, for FP4GroupedLinear
     rows: torch.Tensor  # (tokens, k) int32; -1 where there is no pick
     num_rows: int  # rows of the expert-sorted tensors: enough for any routing of this size
+    # The counts that the row moves go by, in a tensor of their own: `counts` may be changed in place (an all-reduce
+    # over a data-parallel job's ranks) at any time.  A plan with other counts or offsets sets it, or None for `counts`.
+    plan_counts: torch.Tensor | None = None
 
 
 def routed_rows(tokens: int, k: int, experts: int) -> int:
@@ -50,10 +53,12 @@ def _route(logits, k, expert_bias, valid, renormalize):
     dev = logits.device
     weights = torch.empty(tokens, k, dtype=torch.float32, device=dev)
     # Tensors of their own: what a caller does to one in place (an all-reduce of the counts) leaves the others'
-    # versions alone, and the backward reads `share`, which no caller sees, instead of the counts.
+    # versions alone.  The backward reads `share`, which no caller sees, instead of the counts, and the row moves
+    # read `plan_counts`.
     picks = torch.empty(tokens, k, dtype=torch.int32, device=dev)
     rows = torch.empty(tokens, k, dtype=torch.int32, device=dev)
     counts = torch.empty(experts, dtype=torch.int64, device=dev)
+    plan_counts = torch.empty(experts, dtype=torch.int64, device=dev)
     offsets = torch.empty(experts + 1, dtype=torch.int64, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
     share = torch.empty(experts, dtype=torch.float32, device=dev)
@@ -61,23 +66,24 @@ def _route(logits, k, expert_bias, valid, renormalize):
     need = _size(dev, lib.rb_nvfp4_route_workspace, tokens, experts, k)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     tok = _trace.begin("route", logits.numel() * logits.element_size() + 12 * tokens * k)
-    _call(what, dev, lib.rb_nvfp4_route, logits.data_ptr(), code, tokens, experts, ld, k,
+    _call(what, dev, lib.rb_nvfp4_route_plan, logits.data_ptr(), code, tokens, experts, ld, k,
           None if expert_bias is None else expert_bias.data_ptr(), None if valid is None else valid.data_ptr(),
           int(renormalize), weights.data_ptr(), picks.data_ptr(), rows.data_ptr(), counts.data_ptr(),
-          offsets.data_ptr(), loss.data_ptr(), share.data_ptr(), ws.data_ptr(), need)
+          plan_counts.data_ptr(), offsets.data_ptr(), loss.data_ptr(), share.data_ptr(), ws.data_ptr(), need)
     _trace.end(tok)
-    return weights, loss, picks, counts, offsets, rows, share
+    return weights, loss, picks, counts, offsets, rows, plan_counts, share
 
 
 class _RouteFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, expert_bias, valid, renormalize):
         ctx.set_materialize_grads(False)
-        weights, loss, picks, counts, offsets, rows, share = _route(logits, k, expert_bias, valid, renormalize)
-        ctx.mark_non_differentiable(picks, counts, offsets, rows)
+        *out, share = _route(logits, k, expert_bias, valid, renormalize)
+        weights, _, picks = out[:3]
+        ctx.mark_non_differentiable(*out[2:])
         ctx.save_for_backward(logits, weights, picks, share)
         ctx.renormalize = renormalize
-        return weights, loss, picks, counts, offsets, rows
+        return tuple(out)
 
     @staticmethod
     @_first_order
@@ -131,10 +137,11 @@ def route(logits: torch.Tensor, k: int, *, expert_bias: torch.Tensor | None = No
         _like("valid", valid, (tokens,), torch.bool, logits.device, what)
         valid = valid.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        weights, loss, picks, counts, offsets, rows = _RouteFn.apply(logits, k, expert_bias, valid, renormalize)
+        out = _RouteFn.apply(logits, k, expert_bias, valid, renormalize)
     else:
-        weights, loss, picks, counts, offsets, rows, _ = _route(logits, k, expert_bias, valid, renormalize)
-    return Routing(weights, picks, counts, loss, offsets, rows, routed_rows(tokens, k, experts))
+        out = _route(logits, k, expert_bias, valid, renormalize)[:-1]
+    weights, loss, picks, counts, offsets, rows, plan_counts = out
+    return Routing(weights, picks, counts, loss, offsets, rows, routed_rows(tokens, k, experts), plan_counts)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -144,7 +151,7 @@ def route(logits: torch.Tensor, k: int, *, expert_bias: torch.Tensor | None = No
 
 def _plan(r: Routing, device: torch.device, what: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(rows, counts, offsets) of a routing, checked."""
-    rows, counts, offsets = r.rows, r.counts, r.offsets
+    rows, counts, offsets = r.rows, r.counts if r.plan_counts is None else r.plan_counts, r.offsets
     if rows.dtype != torch.int32 or counts.dtype != torch.int64 or offsets.dtype != torch.int64 or rows.dim() != 2 \
             or counts.dim() != 1 or offsets.shape != (counts.shape[0] + 1,):
         raise ValueError(f"{what}: the routing needs int32 rows (tokens, k) and int64 counts (E,) and offsets (E + 1,)")

@@ -1,0 +1,83 @@
+"""What the sublayer operators promise beside their formulas: counts that may be changed in place, derivatives
+that are refused and never dropped, plans that reach past the tensors, types under autocast, accuracy far out."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def nv():
+    import radiance_b200.nvfp4 as nv
+
+    assert nv.nvfp4_supported()
+    return nv
+
+
+def _rand(*shape, dtype=torch.float32, seed=0, std=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, device="cuda", generator=g) * std).to(dtype)
+
+
+def _poison(*shape, dtype=torch.bfloat16):
+    """Leaves NaN in the memory that the next allocations of this size get."""
+    blocks = [torch.full(shape, float("nan"), dtype=dtype, device="cuda") for _ in range(6)]
+    del blocks
+
+
+# ------------------------------------------------------------------------------------------------
+# Counts changed in place between the passes
+# ------------------------------------------------------------------------------------------------
+
+CHANGES = {
+    "sum": lambda c: c.mul_(4),
+    "untracked sum": lambda c: c.data.mul_(4),  # as a collective writes: autograd's version counter stays
+    "untracked mean": lambda c: c.data.div_(3, rounding_mode="floor"),
+    "untracked zero": lambda c: c.data.zero_(),
+}
+
+
+@pytest.mark.parametrize("change", list(CHANGES))
+def test_moves_keep_their_counts(nv, change):
+    """Dispatch, combine and both backwards after an all-reduce of the counts."""
+    x, res = _rand(300, 96, seed=1), _rand(300, 96, seed=3)
+    gy = _rand(300, 96, seed=4)
+
+    def run(first, second):
+        logits, xs_in = _rand(300, 6, seed=2).requires_grad_(), x.clone().requires_grad_()
+        r = nv.route(logits, 2)
+        first(r.counts)
+        _poison(r.num_rows, 96, dtype=torch.float32)
+        xs = nv.token_dispatch(xs_in, r)
+        ys = xs * 2
+        y = nv.token_combine(ys, r, residual=res)
+        second(r.counts)
+        _poison(r.num_rows, 96, dtype=torch.float32)
+        return xs.detach().clone(), y.detach(), *torch.autograd.grad(y, (xs, ys, xs_in, logits), gy)
+
+    want = run(lambda c: None, lambda c: None)
+    for at in ((CHANGES[change], lambda c: None), (lambda c: None, CHANGES[change])):
+        for a, b in zip(run(*at), want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("change", list(CHANGES))
+def test_routed_experts_keep_their_counts(nv, change):
+    """A job that reduces the returned counts before the backward pass gets the gradients of one that does not."""
+    from radiance_b200.nvfp4.grouped import FP4BatchedExperts
+
+    torch.manual_seed(3)
+    ex = FP4BatchedExperts(6, 256, 384, device="cuda")
+    ex.refresh_fp4_cache()
+
+    def run(f):
+        x, logits = _rand(300, 256, dtype=torch.bfloat16, seed=1).requires_grad_(), _rand(300, 6, seed=2).requires_grad_()
+        y, r = ex.forward_routed(x, logits, 2, residual=x)
+        f(r.counts)
+        _poison(r.num_rows, 256)
+        loss = (y.float() * _rand(300, 256, seed=5)).sum() + r.balance_loss
+        return torch.autograd.grad(loss, [x, logits, *ex.parameters()])
+
+    for a, b in zip(run(CHANGES[change]), run(lambda c: None)):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
