@@ -24,6 +24,7 @@ import torch.nn.functional as F
 from .epilogue import (
     _activation_code,
     _dtype_of,
+    _first_order,
     _like,
     _probability,
     _seed_tensor,
@@ -180,6 +181,7 @@ class _FP4EpilogueLinearFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_first_order
     def backward(ctx, grad_y):
         z, seed = ctx.saved_tensors[9:]
         grad_z = grad_y

@@ -81,3 +81,28 @@ def test_routed_experts_keep_their_counts(nv, change):
 
     for a, b in zip(run(CHANGES[change]), run(lambda c: None)):
         assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------------
+# Second derivatives
+# ------------------------------------------------------------------------------------------------
+
+
+def _linear(nv, n=256, k=256, **recipe):
+    torch.manual_seed(1)
+    layer = nv.FP4Linear(k, n, recipe=nv.FP4Recipe(**recipe)).cuda()
+    layer.refresh_fp4_cache()
+    return layer
+
+
+@pytest.mark.parametrize("recipe", [dict(), dict(grad_gemms=False)])
+@pytest.mark.parametrize("act,p", [("gelu", 0.0), (None, 0.0), (None, 0.2), ("silu", 0.1)])
+def test_linear_second_order_is_refused(nv, act, p, recipe):
+    """With residual=x the gradient of x stays differentiable through the residual's part: differentiating it must
+    not silently leave out the linear's."""
+    layer = _linear(nv, **recipe)
+    x = _rand(256, 256, dtype=torch.bfloat16).requires_grad_()
+    y = layer(x, activation=act, dropout_p=p, dropout_seed=3, residual=x)
+    (g,) = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().square().sum().backward()
