@@ -13,7 +13,6 @@ drawn where it is needed and never stored; the three operators draw the same mas
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import _trace
@@ -45,13 +44,33 @@ def _call(what: str, device: torch.device, fn, *args) -> None:
         _lib.check(rc, what)
 
 
+class _Refuse(torch.autograd.Function):
+    """Gradients as they are, which cannot be differentiated again."""
+
+    @staticmethod
+    def forward(ctx, *grads):
+        return grads
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("radiance_b200.nvfp4: these gradients are of first order (once_differentiable) and cannot be "
+                           "differentiated again")
+
+
 def _first_order(backward):
-    """``once_differentiable`` for a Function's backward, entered only where it matters: outside
-    ``create_graph`` grad mode is off already, and its bookkeeping costs as much as a launch."""
-    checked = once_differentiable(backward)
+    """A Function's backward under ``create_graph``: its gradients raise when they are differentiated again.
+    They depend on the upstream gradients, and on the inputs where the forward set ``ctx.curved``; what depends on
+    neither is a constant and stays one.  (torch's ``once_differentiable`` asks for the upstream gradients only.)"""
 
     def wrapper(ctx, *grads):
-        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not (getattr(ctx, "curved", False) or any(g is not None and g.requires_grad for g in grads)):
+            return out
+        refused = iter(_Refuse.apply(*(g.detach().requires_grad_() for g in out if g is not None)))
+        return tuple(None if g is None else next(refused) for g in out)
 
     return wrapper
 

@@ -178,6 +178,9 @@ class _FP4EpilogueLinearFn(torch.autograd.Function):
         # args: weight .. reduce_grad_scale (12), the input's global scale, the wgrad hook
         y = _FP4LinearFn.forward(ctx, x, *args[:12], gemm, args[12], args[13], extra)
         ctx.activation, ctx.dropout_p = activation, dropout_p
+        # The gradients depend on the inputs: through the activation, and x's on the weight and the weight's on x.
+        needs = ctx.needs_input_grad[4:7]
+        ctx.curved = any(needs) if activation is not None else needs[0] and needs[1]
         return y
 
     @staticmethod

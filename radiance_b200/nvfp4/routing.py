@@ -82,7 +82,7 @@ class _RouteFn(torch.autograd.Function):
         weights, _, picks = out[:3]
         ctx.mark_non_differentiable(*out[2:])
         ctx.save_for_backward(logits, weights, picks, share)
-        ctx.renormalize = renormalize
+        ctx.renormalize, ctx.curved = renormalize, True
         return tuple(out)
 
     @staticmethod
@@ -225,6 +225,7 @@ class _CombineFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, residual, rows, counts, offsets):
         ctx.save_for_backward(y, weights, rows, counts, offsets)
+        ctx.curved = ctx.needs_input_grad[0] and ctx.needs_input_grad[1]  # each one's gradient depends on the other
         return _combine(y, rows, weights, residual)
 
     @staticmethod

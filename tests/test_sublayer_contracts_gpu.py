@@ -106,3 +106,38 @@ def test_linear_second_order_is_refused(nv, act, p, recipe):
     (g,) = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.float().square().sum().backward()
+
+
+def _twice(loss, x):
+    """Differentiates a gradient again beside another term that is differentiable twice."""
+    (g,) = torch.autograd.grad(loss + x.float().pow(3).sum(), x, create_graph=True)
+    g.float().square().sum().backward()
+
+
+def test_second_order_under_a_constant_upstream(nv):
+    """Gradients that depend on the inputs are refused even where the upstream gradient is a constant."""
+    layer, x = _linear(nv), _rand(256, 256, dtype=torch.bfloat16).requires_grad_()
+    for kw in (dict(activation="gelu"), dict(residual=x), dict(dropout_p=0.1, dropout_seed=1)):
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            _twice(layer(x, **kw).float().sum(), x)
+    logits = _rand(200, 6).requires_grad_()
+    for pick in (lambda r: r.balance_loss, lambda r: r.weights[:, 0].sum()):
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            _twice(pick(nv.route(logits, 2)), logits)
+    r = nv.route(logits, 2)
+    y = _rand(r.num_rows, 16).requires_grad_()
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        _twice(nv.token_combine(y, r).sum(), y)
+
+
+def test_constant_gradients_stay_constants(nv):
+    """A linear map's gradient under a constant upstream is a constant, and what multiplies it may be differentiated."""
+    x = _rand(200, 16).requires_grad_()
+    r = nv.route(_rand(200, 6), 2)
+    y = _rand(r.num_rows, 16).requires_grad_()
+    for f, v in ((lambda v: nv.dropout(v, 0.4, seed=3), x), (lambda v: nv.token_dispatch(v, r), x),
+                 (lambda v: nv.token_combine(v, r), y)):
+        (g,) = torch.autograd.grad(f(v).sum(), v, create_graph=True)
+        assert not g.requires_grad
+        (got,) = torch.autograd.grad((g * v).sum(), v)
+        assert torch.equal(got, g)
