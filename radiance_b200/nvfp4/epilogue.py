@@ -13,6 +13,7 @@ drawn where it is needed and never stored; the three operators draw the same mas
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from . import _trace
@@ -42,6 +43,13 @@ def _call(what: str, device: torch.device, fn, *args) -> None:
             rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, what)
+
+
+def _tracked(*tensors: torch.Tensor | None) -> bool:
+    """Whether autograd follows one of these: in reverse (it requires a gradient) or forward mode (it has a tangent)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _Refuse(torch.autograd.Function):
@@ -181,7 +189,7 @@ def dropout(x: torch.Tensor, p: float = 0.5, *, seed: torch.Tensor | int | None 
     if p == 0.0 and residual is None:
         return x
     seed = _seed_tensor(seed, x.device, what) if p > 0.0 else None
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    if _tracked(x, residual):
         return _DropoutFn.apply(x, residual, p, seed)
     return _dropout(x, residual, p, seed)
 

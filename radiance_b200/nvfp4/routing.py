@@ -17,7 +17,7 @@ import torch
 
 from .. import _lib
 from . import _trace
-from .epilogue import _call, _dtype_of, _first_order, _like, _rows, _size
+from .epilogue import _call, _dtype_of, _first_order, _like, _rows, _size, _tracked
 from .quantize import _require_cuda
 
 MAX_EXPERTS = 256  # the grouped GEMM's group limit
@@ -136,7 +136,7 @@ def route(logits: torch.Tensor, k: int, *, expert_bias: torch.Tensor | None = No
     if valid is not None:
         _like("valid", valid, (tokens,), torch.bool, logits.device, what)
         valid = valid.contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _tracked(logits):
         out = _RouteFn.apply(logits, k, expert_bias, valid, renormalize)
     else:
         out = _route(logits, k, expert_bias, valid, renormalize)[:-1]
@@ -248,7 +248,7 @@ def token_dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     rows, counts, offsets = _plan(routing, x.device, what)
     if x.dim() != 2 or x.shape[0] != rows.shape[0] or x.shape[1] < 1:
         raise ValueError(f"{what}: rows of shape ({rows.shape[0]}, d) expected, got {tuple(x.shape)}")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _tracked(x):
         return _DispatchFn.apply(x, rows, counts, offsets, routing.num_rows)
     return _dispatch(x, rows, counts, offsets, routing.num_rows)
 
@@ -270,7 +270,6 @@ def token_combine(y: torch.Tensor, routing: Routing, *, residual: torch.Tensor |
     weights = weights.contiguous()
     if residual is not None:
         _like("residual", residual, (tokens, y.shape[1]), y.dtype, y.device, what)
-    if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
+    if _tracked(y, weights, residual):
         return _CombineFn.apply(y, weights, residual, rows, counts, offsets)
     return _combine(y, rows, weights, residual)

@@ -141,3 +141,36 @@ def test_constant_gradients_stay_constants(nv):
         assert not g.requires_grad
         (got,) = torch.autograd.grad((g * v).sum(), v)
         assert torch.equal(got, g)
+
+
+# ------------------------------------------------------------------------------------------------
+# Forward mode
+# ------------------------------------------------------------------------------------------------
+
+
+def test_tangents_are_refused_not_dropped(nv):
+    """There are no forward-mode formulas: a dual tensor raises, and other tensors work beside one."""
+    from torch.autograd import forward_ad
+
+    layer, x = _linear(nv), _rand(256, 256, dtype=torch.bfloat16)
+    logits = _rand(256, 6)
+    r = nv.route(logits, 2)
+    y = _rand(r.num_rows, 256, dtype=torch.bfloat16)
+    calls = {
+        "dropout": (lambda v: nv.dropout(v, 0.5, seed=1), x),
+        "dropout residual": (lambda v: nv.dropout(x, 0.5, seed=1, residual=v), x),
+        "linear": (lambda v: layer(v, activation="gelu"), x),
+        "linear residual": (lambda v: layer(x, residual=v), x),
+        "route": (lambda v: nv.route(v, 2).weights, logits),
+        "dispatch": (lambda v: nv.token_dispatch(v, r), x),
+        "combine": (lambda v: nv.token_combine(v, r), y),
+        "combine weights": (lambda v: nv.token_combine(y, r._replace(weights=v)), r.weights),
+        "combine residual": (lambda v: nv.token_combine(y, r, residual=v), x),
+    }
+    for name, (f, v) in calls.items():
+        want = f(v)
+        with forward_ad.dual_level():
+            assert torch.equal(f(v), want), name
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    f(forward_ad.make_dual(v, torch.ones_like(v)))
