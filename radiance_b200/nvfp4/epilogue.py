@@ -65,6 +65,30 @@ class _Refuse(torch.autograd.Function):
                            "differentiated again")
 
 
+class _NoGradient(torch.autograd.Function):
+    """A call without a gradient formula on tensors that autograd follows: its results raise in backward, as those
+    of ``mm`` do, instead of being taken for constants."""
+
+    @staticmethod
+    def forward(ctx, what, call, kwargs, *tensors):
+        ctx.set_materialize_grads(False)
+        ctx.what = what
+        return call(*tensors, **kwargs)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what} has no gradient formula: FP4Linear differentiates it")
+
+
+def _functional(what: str, call, out: torch.Tensor | None, kwargs, *tensors):
+    """``call(*tensors, out=out, **kwargs)``, refused or without a gradient where autograd follows a tensor."""
+    if not _tracked(out, *tensors):
+        return call(*tensors, out=out, **kwargs)
+    if out is not None:
+        raise ValueError(f"{what}: out= cannot be differentiated, and one of its tensors requires a gradient")
+    return _NoGradient.apply(what, call, dict(kwargs, out=None), *tensors)
+
+
 def _first_order(backward):
     """A Function's backward under ``create_graph``: its gradients raise when they are differentiated again.
     They depend on the upstream gradients, and on the inputs where the forward set ``ctx.curved``; what depends on
@@ -252,8 +276,15 @@ def epilogue_mm(a: NVFP4Tensor, b: NVFP4Tensor, *, bias: torch.Tensor | None = N
     (erf) or "gelu_tanh".  ``dropout_p`` and ``seed`` as in ``dropout`` (None: a fresh seed; a backward
     pass needs the seed, so keep it).  ``residual``: ``(M, N)`` of ``out_dtype``.  ``out`` may be the
     residual itself.  With ``save_preact`` also returns ``z`` in ``out_dtype``, which
-    ``epilogue_backward`` takes.
+    ``epilogue_backward`` takes.  No gradient formula (``FP4Linear`` has one): where ``bias`` or ``residual``
+    requires a gradient, the result raises in backward, and ``out`` is refused.
     """
+    return _functional("nvfp4.epilogue_mm", _epilogue_mm, out,
+                       dict(a=a, b=b, activation=activation, dropout_p=dropout_p, seed=seed, out_dtype=out_dtype,
+                            save_preact=save_preact), bias, residual)
+
+
+def _epilogue_mm(bias, residual, *, a, b, activation, dropout_p, seed, out_dtype, out, save_preact):
     what = "nvfp4.epilogue_mm"
     ap, bp = a.packed, b.packed
     _require_cuda(ap, what)
@@ -313,8 +344,13 @@ def epilogue_backward(grad_y: torch.Tensor, preact: torch.Tensor | None = None, 
     One pass over ``grad_y`` and ``preact`` (2-D, the same dtype) that also takes the global scale of
     ``grad_z``, which the quantizer of the backward GEMMs needs, and with ``bias_grad`` its fp32 column
     sums.  ``seed`` is the forward call's.  Returns ``(grad_z, global_scale_of(grad_z), sums or None)``.
-    The gradient of the residual is ``grad_y`` itself.
+    The gradient of the residual is ``grad_y`` itself.  No gradient formula, as ``epilogue_mm``.
     """
+    return _functional("nvfp4.epilogue_backward", _epilogue_backward, out,
+                       dict(activation=activation, dropout_p=dropout_p, seed=seed, bias_grad=bias_grad), grad_y, preact)
+
+
+def _epilogue_backward(grad_y, preact, *, activation, dropout_p, seed, bias_grad, out):
     what = "nvfp4.epilogue_backward"
     _require_cuda(grad_y, what)
     code, act = _dtype_of(grad_y, what), _activation_code(activation, what)

@@ -174,3 +174,48 @@ def test_tangents_are_refused_not_dropped(nv):
             for grad in (True, False):
                 with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
                     f(forward_ad.make_dual(v, torch.ones_like(v)))
+
+
+# ------------------------------------------------------------------------------------------------
+# Functional forms without a gradient
+# ------------------------------------------------------------------------------------------------
+
+
+def test_functional_forms_say_that_they_have_no_gradient(nv):
+    """A bias, residual or gradient that requires a gradient is no constant: the result raises in backward."""
+    from torch.autograd import forward_ad
+
+    qa, qb = nv.quantize(_rand(256, 128, seed=1), -1), nv.quantize(_rand(384, 128, seed=2), -1)
+    bias, res = _rand(384, seed=3), _rand(256, 384, seed=4)
+    kw = dict(activation="silu", out_dtype=torch.float32)
+    want, wz = nv.epilogue_mm(qa, qb, bias=bias, residual=res, save_preact=True, **kw)
+    for name in ("bias", "residual"):
+        args = dict(bias=bias, residual=res)
+        args[name] = args[name].clone().requires_grad_()
+        y, z = nv.epilogue_mm(qa, qb, save_preact=True, **args, **kw)
+        assert torch.equal(y, want) and torch.equal(z, wz)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            y.sum().backward()
+        with pytest.raises(ValueError, match="out="):
+            nv.epilogue_mm(qa, qb, out=torch.empty_like(want), **args, **kw)
+        with torch.no_grad():
+            out = torch.empty_like(want)
+            assert nv.epilogue_mm(qa, qb, out=out, **args, **kw) is out and torch.equal(out, want)
+            assert not nv.epilogue_mm(qa, qb, **args, **kw).requires_grad
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+            args[name] = forward_ad.make_dual(args[name].detach(), torch.ones_like(args[name]))
+            nv.epilogue_mm(qa, qb, **args, **kw)
+    leaf = torch.zeros_like(want).requires_grad_()
+    with pytest.raises(ValueError, match="out="):
+        nv.epilogue_mm(qa, qb, bias=bias, residual=res, out=leaf, **kw)
+    gy = _rand(256, 384, seed=5)
+    gz, gs, sums = nv.epilogue_backward(gy, wz, activation="silu", bias_grad=True)
+    for g, z in ((gy.clone().requires_grad_(), wz), (gy, wz.clone().requires_grad_())):
+        got = nv.epilogue_backward(g, z, activation="silu", bias_grad=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, (gz, gs, sums)))
+        with pytest.raises(RuntimeError, match="no gradient"):
+            got[0].sum().backward()
+        got = nv.epilogue_backward(g, z, activation="silu")
+        assert torch.equal(got[0], gz) and got[2] is None
+        with pytest.raises(ValueError, match="out="):
+            nv.epilogue_backward(g, z, activation="silu", out=torch.empty_like(gz))
