@@ -83,7 +83,10 @@ class _NoGradient(torch.autograd.Function):
 def _functional(what: str, call, out: torch.Tensor | None, kwargs, *tensors):
     """``call(*tensors, out=out, **kwargs)``, refused or without a gradient where autograd follows a tensor."""
     if not _tracked(out, *tensors):
-        return call(*tensors, out=out, **kwargs)
+        result = call(*tensors, out=out, **kwargs)
+        if out is not None:  # written behind autograd's back: whoever saved it for backward must learn of it
+            torch.autograd.graph.increment_version(out)
+        return result
     if out is not None:
         raise ValueError(f"{what}: out= cannot be differentiated, and one of its tensors requires a gradient")
     return _NoGradient.apply(what, call, dict(kwargs, out=None), *tensors)

@@ -219,3 +219,20 @@ def test_functional_forms_say_that_they_have_no_gradient(nv):
         assert torch.equal(got[0], gz) and got[2] is None
         with pytest.raises(ValueError, match="out="):
             nv.epilogue_backward(g, z, activation="silu", out=torch.empty_like(gz))
+
+
+def test_writing_to_out_is_seen_by_autograd(nv):
+    """A tensor that another op saved for its backward and that out= then overwrites: backward raises."""
+    qa, qb = nv.quantize(_rand(256, 128, seed=1), -1), nv.quantize(_rand(256, 128, seed=2), -1)
+    calls = (lambda t: nv.epilogue_mm(qa, qb, residual=t, out=t, out_dtype=torch.float32),
+             lambda t: nv.epilogue_mm(qa, qb, out=t, out_dtype=torch.float32),
+             lambda t: nv.epilogue_backward(t, dropout_p=0.5, seed=1, out=t))
+    for call in calls:
+        w, stream = _rand(256, 256, seed=3).requires_grad_(), _rand(256, 256, seed=4)
+        loss = (w * stream).sum()
+        call(stream)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():  # tensors without a version counter
+        t = _rand(256, 256, seed=4)
+        calls[0](t)
