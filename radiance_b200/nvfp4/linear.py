@@ -320,7 +320,7 @@ class FP4Linear(nn.Linear):
             y = F.linear(x, self.weight.to(x.dtype), None if self.bias is None else self.bias.to(x.dtype))
             if plain:
                 return y
-            y = _TORCH_ACTIVATIONS[activation](y)
+            y = _TORCH_ACTIVATIONS[activation](y.to(x.dtype))  # autocast's product is bf16, the FP4 path's output x's type
             return dropout(y, dropout_p, seed=dropout_seed, residual=residual)
         flat = x.reshape(-1, self.in_features).contiguous()
         if plain:

@@ -236,3 +236,23 @@ def test_writing_to_out_is_seen_by_autograd(nv):
     with torch.inference_mode():  # tensors without a version counter
         t = _rand(256, 256, seed=4)
         calls[0](t)
+
+
+# ------------------------------------------------------------------------------------------------
+# Autocast
+# ------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("tokens", [256, 100])  # NVFP4 and the bf16 fallback
+@pytest.mark.parametrize("kw", [dict(), dict(activation="gelu"), dict(activation="silu", dropout_p=0.1, dropout_seed=2)])
+def test_linear_keeps_its_type_under_autocast(nv, tokens, kw):
+    """An fp32 stream under bf16 autocast: the residual has the input's type on either path, and so has the output."""
+    layer = _linear(nv)
+    x, res = _rand(tokens, 256, seed=1).requires_grad_(), _rand(tokens, 256, seed=2).requires_grad_()
+    with torch.autocast("cuda", torch.bfloat16):
+        y = layer(x, residual=res, **kw)
+        if kw:
+            assert layer(x, **kw).dtype == torch.float32
+    assert y.dtype == torch.float32
+    gx, gr = torch.autograd.grad(y, (x, res), torch.ones_like(y))
+    assert torch.isfinite(gx).all() and (gr == 1).all()
