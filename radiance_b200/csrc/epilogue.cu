@@ -268,13 +268,15 @@ int check_common(const char* what, int dtype, double p, const int64_t* seed) {
 
 // Row splits of the backward kernel: one wave of the blocks that an SM holds at once (one block
 // more than that and the last ones run alone), each with at least 16 rows.
-int64_t backward_parts(int64_t rows, int64_t gx) {
-  const int64_t want = (int64_t)rb::kBwdBlocksPerSm * rb_host::sm_budget(rb_host::current_device()) / gx;
+int64_t backward_parts(int64_t rows, int64_t gx, int sms) {
+  const int64_t want = (int64_t)rb::kBwdBlocksPerSm * sms / gx;
   const int64_t most = (rows + 15) / 16;
   int64_t parts = want < most ? want : most;
   if (parts > 65535) parts = 65535;
   return parts < 1 ? 1 : parts;
 }
+
+size_t backward_scratch(int64_t parts, int64_t cols, int64_t gx) { return (size_t)(parts * cols + parts * gx) * 4; }
 
 }  // namespace
 
@@ -319,8 +321,9 @@ int rb_nvfp4_dropout(const void* x, const void* residual, int dtype, int64_t n, 
 
 size_t rb_nvfp4_epilogue_backward_workspace(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  const int64_t gx = (cols + 255) / 256, parts = backward_parts(rows, gx);
-  return (size_t)(parts * cols + parts * gx) * 4;
+  // Enough for every SM budget (another thread may change it before the call): the splits grow with the SMs.
+  const int64_t gx = (cols + 255) / 256;
+  return backward_scratch(backward_parts(rows, gx, rb_host::num_sms(rb_host::current_device())), cols, gx);
 }
 
 int rb_nvfp4_epilogue_backward(const void* grad_y, int64_t ldg, const void* preact, int64_t ldz, int dtype,
@@ -345,7 +348,9 @@ int rb_nvfp4_epilogue_backward(const void* grad_y, int64_t ldg, const void* prea
     return RB_ERR_ARG;
   }
   if (!on_sm100(what)) return RB_ERR_DEVICE;
-  if (workspace_bytes < rb_nvfp4_epilogue_backward_workspace(rows, cols)) {
+  const int64_t gx = (cols + 255) / 256;
+  int64_t parts = backward_parts(rows, gx, rb_host::sm_budget(rb_host::current_device()));
+  if (workspace_bytes < backward_scratch(parts, cols, gx)) {
     rb_host::set_error("%s: a workspace of %zu bytes is too small", what, workspace_bytes);
     return RB_ERR_ARG;
   }
@@ -359,8 +364,6 @@ int rb_nvfp4_epilogue_backward(const void* grad_y, int64_t ldg, const void* prea
   a.ldz = ldz;
   a.ldo = ldo;
   a.drop = rb_host::dropout_args(p, seed);
-  const int64_t gx = (cols + 255) / 256;
-  int64_t parts = backward_parts(rows, gx);
   if (gx > 0x7FFFFFFF) {
     rb_host::set_error("%s: tensor too wide", what);
     return RB_ERR_SHAPE;

@@ -2,6 +2,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "common.cuh"
@@ -46,19 +47,18 @@ int num_sms(int device) {
   return cache[device];
 }
 
-static int g_sm_budget[64] = {0};
+static std::atomic<int> g_sm_budget[64];
 
 int sm_budget(int device) {
   const int n = num_sms(device);
-  if (device < 0 || device >= 64 || g_sm_budget[device] <= 0 || g_sm_budget[device] >= n) return n;
-  return g_sm_budget[device];
+  if (device < 0 || device >= 64) return n;
+  const int b = g_sm_budget[device].load(std::memory_order_relaxed);  // once: another thread may set it
+  return b <= 0 || b >= n ? n : b;
 }
 
 int set_sm_budget(int device, int sms) {
   if (device < 0 || device >= 64) return 0;
-  const int prev = g_sm_budget[device];
-  g_sm_budget[device] = sms < 0 ? 0 : sms;
-  return prev;
+  return g_sm_budget[device].exchange(sms < 0 ? 0 : sms, std::memory_order_relaxed);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {

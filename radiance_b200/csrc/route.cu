@@ -837,9 +837,8 @@ int route_lanes(int experts) {
 
 // Tokens per block: the same for every SM, in whole steps of the block's token groups, and no more pairs than
 // its shared memory holds.
-int64_t route_chunk(int64_t tokens, int experts, int k) {
+int64_t route_chunk(int64_t tokens, int experts, int k, int64_t sms) {
   const int groups = rb::kRouteThreads / route_lanes(experts);
-  const int64_t sms = rb_host::sm_budget(rb_host::current_device());
   const int64_t most = rb::kMaxPairs / k;
   const int64_t turns = (tokens + sms * most - 1) / (sms * most);  // blocks per SM
   int64_t c = turns > 0 ? (tokens + sms * turns - 1) / (sms * turns) : 1;
@@ -847,6 +846,8 @@ int64_t route_chunk(int64_t tokens, int experts, int k) {
   if (c > most) c = most;
   return c < 1 ? 1 : c;
 }
+
+size_t route_scratch(int64_t blocks, int64_t experts) { return (size_t)(blocks * (6 * experts + 4)); }
 
 // f(LPT, ITEMS) as integral constants for the number of experts.
 template <typename F>
@@ -938,9 +939,15 @@ extern "C" {
 
 size_t rb_nvfp4_route_workspace(int64_t tokens, int64_t experts, int k) {
   if (tokens < 0 || experts < 1 || experts > rb::kMaxExperts || k < 1 || k > rb::kMaxTopK) return 0;
-  const int64_t chunk = route_chunk(tokens, (int)experts, k);
-  const int64_t blocks = tokens > 0 ? (tokens + chunk - 1) / chunk : 1;
-  return (size_t)(blocks * (6 * experts + 4));
+  // Enough for every SM budget, which another thread may change before the call that uses it.  With s SMs a chunk
+  // has at least tokens / (s turns) tokens, turns < tokens / (s most) + 1, or is `most`: never more than
+  // s + tokens / most blocks.  And it is never below a step of the block's groups (or `most`).
+  const int64_t most = rb::kMaxPairs / k, step = rb::kRouteThreads / route_lanes((int)experts);
+  const int64_t least = step < most ? step : most;
+  const int64_t a = rb_host::num_sms(rb_host::current_device()) + (tokens + most - 1) / most;
+  const int64_t b = (tokens + least - 1) / least;
+  const int64_t blocks = a < b ? a : b;
+  return route_scratch(blocks > 1 ? blocks : 1, experts);
 }
 
 int rb_nvfp4_route_plan(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int k,
@@ -954,7 +961,10 @@ int rb_nvfp4_route_plan(const void* logits, int dtype, int64_t tokens, int64_t e
       unaligned(counts, 8) || unaligned(plan_counts, 8) || unaligned(offsets, 8) || unaligned(workspace, 4))
     return route_failed(RB_ERR_ARG, "%s: null or misaligned pointer argument", what);
   if (!route_device(what)) return RB_ERR_DEVICE;
-  if (workspace_bytes < rb_nvfp4_route_workspace(tokens, experts, k))
+  const int64_t sms = rb_host::sm_budget(rb_host::current_device());
+  const int64_t chunk = route_chunk(tokens, (int)experts, k, sms);
+  const int64_t blocks = tokens > 0 ? (tokens + chunk - 1) / chunk : 1;
+  if (workspace_bytes < route_scratch(blocks, experts))
     return route_failed(RB_ERR_ARG, "%s: a workspace of %lld bytes is too small", what, (long long)workspace_bytes);
   rb::RouteArgs a = {};
   a.logits = logits;
@@ -973,8 +983,8 @@ int rb_nvfp4_route_plan(const void* logits, int dtype, int64_t tokens, int64_t e
   a.offsets = offsets;
   a.loss = loss;
   a.share = share;
-  a.chunk = route_chunk(tokens, a.experts, k);
-  a.blocks = tokens > 0 ? (tokens + a.chunk - 1) / a.chunk : 1;
+  a.chunk = chunk;
+  a.blocks = blocks;
   a.psum = reinterpret_cast<float*>(workspace);
   a.nrouted = reinterpret_cast<int32_t*>(a.psum + a.blocks * experts);
   a.hist = reinterpret_cast<uint16_t*>(a.nrouted + a.blocks);
@@ -988,7 +998,6 @@ int rb_nvfp4_route_plan(const void* logits, int dtype, int64_t tokens, int64_t e
           <<<(unsigned)a.blocks, rb::kRouteThreads, 0, st>>>(a);
   });
   if (a.blocks > 1) {
-    const int sms = rb_host::sm_budget(rb_host::current_device());
     const unsigned workers = (unsigned)(a.blocks < sms ? a.blocks : sms);
     rb::route_plan_kernel<<<workers + 1, rb::kRouteThreads, 0, st>>>(a);
   }

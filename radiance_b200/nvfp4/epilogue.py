@@ -111,7 +111,7 @@ def _first_order(backward):
 
 
 def _size(device: torch.device, fn, *args) -> int:
-    """A workspace size, asked with ``device`` current (it goes by the device's SMs and its budget)."""
+    """A workspace size, asked with ``device`` current (it goes by the device's SMs)."""
     if device.index == torch.cuda.current_device():
         return int(fn(*args))
     with torch.cuda.device(device):

@@ -256,3 +256,40 @@ def test_linear_keeps_its_type_under_autocast(nv, tokens, kw):
     assert y.dtype == torch.float32
     gx, gr = torch.autograd.grad(y, (x, res), torch.ones_like(y))
     assert torch.isfinite(gx).all() and (gr == 1).all()
+
+
+# ------------------------------------------------------------------------------------------------
+# Another thread's SM budget
+# ------------------------------------------------------------------------------------------------
+
+
+def test_sm_budget_may_change_between_and_during_calls(nv):
+    """Workspaces hold whatever budget another thread sets meanwhile; picks, plans and gradients do not depend on it."""
+    import threading
+
+    from radiance_b200 import _lib
+
+    logits, gy, z = _rand(20000, 64, seed=1), _rand(2000, 520, seed=2), _rand(2000, 520, seed=3)
+    want, wz = nv.route(logits, 4), nv.epilogue_backward(gy, z, activation="silu", bias_grad=True)
+    stop = threading.Event()
+
+    def toggle():
+        while not stop.is_set():
+            for sms in (1, 148, 7, 0, 90):
+                _lib.set_sm_budget(sms)
+
+    before = _lib.set_sm_budget(0)
+    thread = threading.Thread(target=toggle)
+    thread.start()
+    try:
+        for _ in range(200):
+            r, got = nv.route(logits, 4), nv.epilogue_backward(gy, z, activation="silu", bias_grad=True)
+            for a, b in ((r.experts, want.experts), (r.rows, want.rows), (r.counts, want.counts),
+                         (r.weights, want.weights), (got[0], wz[0]), (got[1], wz[1])):
+                assert torch.equal(a, b)
+            # fp32 sums of 2000 terms in another order
+            assert ((got[2] - wz[2]).abs() <= 2000 * 2.0**-23 * wz[0].abs().sum(0)).all()
+    finally:
+        stop.set()
+        thread.join()
+        _lib.set_sm_budget(before)
