@@ -68,7 +68,7 @@ int rb_nvfp4_abi_version(void);
  * streaming multiprocessors (0 = all of them), so that kernels of another stream -- a gradient
  * reduce-scatter overlapping the backward pass -- find SMs free while ours run.  Returns the previous
  * budget.  Host-side setting for the launches that follow; any thread may set it at any time: no call
- * reads it twice for one layout, and the workspace of the epilogue's backward and of the routing does not depend on it.  No counterpart in the reference.
+ * reads it twice for one layout, and no workspace size depends on it.  No counterpart in the reference.
  */
 int rb_nvfp4_set_sm_budget(int sms);
 

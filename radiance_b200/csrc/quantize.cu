@@ -1581,8 +1581,8 @@ int rb_nvfp4_quantize_grouped(const void* x, int dtype, int64_t rows, int64_t co
 
 // Row splits of global_scale_colsum_kernel for a launch of `gx` column chunks: enough blocks to
 // fill the GPU four times over, and at most one per row.
-static int64_t colsum_parts(int64_t rows, int64_t gx) {
-  const int64_t want = (4 * (int64_t)rb_host::sm_budget(rb_host::current_device()) + gx - 1) / gx;
+static int64_t colsum_parts(int64_t rows, int64_t gx, int sms) {
+  const int64_t want = (4 * (int64_t)sms + gx - 1) / gx;
   return max((int64_t)1, min(rows, want));
 }
 
@@ -1590,7 +1590,8 @@ size_t rb_nvfp4_global_scale_colsum_workspace(int dtype, int64_t rows, int64_t c
   if (rows <= 0 || cols <= 0) return 16;
   const int64_t per_block = (dtype == RB_DTYPE_F32 ? 4 : 8) * 256;
   const int64_t gx = (cols + per_block - 1) / per_block;
-  return 16 + (size_t)colsum_parts(rows, gx) * (size_t)cols * sizeof(float);
+  // Enough for every SM budget (another thread may change it before the call): the splits grow with the SMs.
+  return 16 + (size_t)colsum_parts(rows, gx, rb_host::num_sms(rb_host::current_device())) * (size_t)cols * sizeof(float);
 }
 
 int rb_nvfp4_global_scale_colsum(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, float* gs_out,
@@ -1618,7 +1619,7 @@ int rb_nvfp4_global_scale_colsum(const void* x, int dtype, int64_t rows, int64_t
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int64_t per_block = (int64_t)(16 / esize) * 256;
   const int64_t gx = (cols + per_block - 1) / per_block;
-  const int64_t parts = colsum_parts(rows, gx);
+  const int64_t parts = colsum_parts(rows, gx, rb_host::sm_budget(rb_host::current_device()));
   if (gx > 0x7FFFFFFF || parts > 65535) {
     rb_host::set_error("nvfp4 global_scale_colsum: tensor too large");
     return RB_ERR_SHAPE;

@@ -42,6 +42,8 @@ def test_workspaces_hold_for_every_sm_budget():
              for t, e, k in ((0, 8, 2), (1, 1, 1), (4099, 160, 6), (16384, 8, 2), (131072, 64, 8), (300, 256, 32))]
     sizes += [(lambda r=r, c=c: lib.rb_nvfp4_epilogue_backward_workspace(r, c))
               for r, c in ((1, 1), (640, 1152), (16384, 5632), (17, 40000), (1 << 22, 8))]
+    sizes += [(lambda d=d, r=r, c=c: lib.rb_nvfp4_global_scale_colsum_workspace(d, r, c))
+              for d, r, c in ((0, 16384, 5632), (1, 640, 1152), (0, 1 << 20, 64))]
     before = _lib.set_sm_budget(0)
     try:
         full = [f() for f in sizes]
