@@ -792,7 +792,8 @@ struct Gemm2Smem {
   uint64_t acc_empty;               // leader: the pair's epilogue warps are done with the shared columns
   uint64_t drain;
   uint64_t res_full[Gemm2Cfg<kMode>::kIsFused ? Gemm2Cfg<kMode>::kOutBoxes : 1];  // fused: a residual has landed
-  float bias[Gemm2Cfg<kMode>::kIsFused ? Gemm2Cfg<kMode>::kEpiWarps : 1][kEpiChunk];  // fused: a chunk's, per warp
+  // fused: a chunk's, per warp; read in vectors of four
+  alignas(16) float bias[Gemm2Cfg<kMode>::kIsFused ? Gemm2Cfg<kMode>::kEpiWarps : 1][kEpiChunk];
   uint32_t tmem_base;
 };
 
