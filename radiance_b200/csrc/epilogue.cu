@@ -23,13 +23,21 @@ namespace rb {
 // and time, 35 and 42 us.
 constexpr int kDropoutBlocksPerSm = 5;
 
-// Eight elements as loaded.
+// Eight elements as loaded.  Coherent loads, not the read-only path: the output may be the input itself.  Dropout of
+// bf16, where a warp reads whole lines, passes L1 by (kL2: 16384 x 2048 with a residual 33.9 us against 34.8, 16384 x
+// 5632 72.4 against 75.5); fp32's two vectors a thread (73.5 us against 69.6) and the epilogue's backward (without an
+// activation 64.5 us against 63.1) take it.
 template <typename T>
 struct Raw8 {
   uint4 q[sizeof(T) / 2];
+  template <bool kL2 = false>
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) q[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) {
+      const uint4* at = reinterpret_cast<const uint4*>(p) + i;
+      if constexpr (kL2) q[i] = __ldcg(at);
+      else q[i] = *at;
+    }
   }
   __device__ __forceinline__ void get(float2 (&v)[4]) const {
     const uint32_t* w = reinterpret_cast<const uint32_t*>(q);
@@ -48,14 +56,15 @@ __global__ void __launch_bounds__(256, kDropoutBlocksPerSm) dropout_kernel(const
   const int64_t step = (int64_t)gridDim.x * blockDim.x, first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t groups = kVec ? n / 8 : 0;
   if (kVec && first < groups) {
+    constexpr bool kL2 = sizeof(T) == 2;
     Raw8<T> xn, rn;
-    xn.load(x + 8 * first);
-    if constexpr (kResidual) rn.load(residual + 8 * first);
+    xn.template load<kL2>(x + 8 * first);
+    if constexpr (kResidual) rn.template load<kL2>(residual + 8 * first);
     for (int64_t g = first; g < groups; g += step) {
       const Raw8<T> xc = xn, rc = rn;
       if (g + step < groups) {
-        xn.load(x + 8 * (g + step));
-        if constexpr (kResidual) rn.load(residual + 8 * (g + step));
+        xn.template load<kL2>(x + 8 * (g + step));
+        if constexpr (kResidual) rn.template load<kL2>(residual + 8 * (g + step));
       }
       float2 v[4];
       xc.get(v);

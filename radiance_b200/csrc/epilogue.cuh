@@ -213,12 +213,6 @@ struct Io;
 
 template <>
 struct Io<__nv_bfloat16> {
-  static __device__ __forceinline__ void load8(float2 (&v)[4], const __nv_bfloat16* p) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
-  }
   // Returns the largest magnitude stored, as fp32 bits (NaN above infinity).
   static __device__ __forceinline__ uint32_t store8(__nv_bfloat16* p, const float2 (&v)[4]) {
     uint32_t w[4], m = 0;
@@ -241,11 +235,6 @@ struct Io<__nv_bfloat16> {
 
 template <>
 struct Io<float> {
-  static __device__ __forceinline__ void load8(float2 (&v)[4], const float* p) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w);
-    v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
-  }
   static __device__ __forceinline__ uint32_t store8(float* p, const float2 (&v)[4]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
     reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);

@@ -293,3 +293,40 @@ def test_sm_budget_may_change_between_and_during_calls(nv):
         stop.set()
         thread.join()
         _lib.set_sm_budget(before)
+
+
+# ------------------------------------------------------------------------------------------------
+# In place
+# ------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [1 << 22, (1 << 22) + 5])
+def test_dropout_in_place(nv, n, dtype):
+    """The C entry with y = x and with y = residual, more elements than one round of the blocks takes."""
+    from radiance_b200 import _lib
+
+    lib = _lib.load()
+    x, res, seed = _rand(n, dtype=dtype, seed=1), _rand(n, dtype=dtype, seed=2), torch.tensor(7, device="cuda")
+    code = {torch.bfloat16: _lib.RB_DTYPE_BF16, torch.float32: _lib.RB_DTYPE_F32}[dtype]
+    stream = torch.cuda.current_stream().cuda_stream
+    for r in (None, res):
+        want = nv.dropout(x, 0.3, seed=seed, residual=r)
+        for into_x in (True, False) if r is not None else (True,):
+            a, b = x.clone(), res.clone()
+            y = a if into_x else b
+            _lib.check(lib.rb_nvfp4_dropout(a.data_ptr(), None if r is None else b.data_ptr(), code, n, 0.3,
+                                            seed.data_ptr(), y.data_ptr(), stream), "dropout")
+            assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cols", [1024, 1021])
+def test_epilogue_backward_into_its_inputs(nv, cols, dtype):
+    gy, z = _rand(3000, cols, dtype=dtype, seed=1), _rand(3000, cols, dtype=dtype, seed=2)
+    kw = dict(activation="gelu", dropout_p=0.2, seed=5, bias_grad=True)
+    want = nv.epilogue_backward(gy, z, **kw)
+    for into_gradient in (True, False):
+        a, b = gy.clone(), z.clone()
+        got = nv.epilogue_backward(a, b, out=a if into_gradient else b, **kw)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
