@@ -330,3 +330,62 @@ def test_epilogue_backward_into_its_inputs(nv, cols, dtype):
         a, b = gy.clone(), z.clone()
         got = nv.epilogue_backward(a, b, out=a if into_gradient else b, **kw)
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------------
+# Plans that reach past the tensors
+# ------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 61])
+def test_a_wrong_plan_writes_nothing_outside(nv, d, dtype):
+    """Rows just past the layout, far past it and below it are skipped, padding ranges are cut to the tensor: the
+    rows around it keep what they held, and the pairs that lie inside it their results."""
+    from radiance_b200 import _lib
+
+    lib = _lib.load()
+    code = {torch.bfloat16: _lib.RB_DTYPE_BF16, torch.float32: _lib.RB_DTYPE_F32}[dtype]
+    stream = torch.cuda.current_stream().cuda_stream
+    r = nv.route(_rand(40, 4, seed=1), 2)
+    n, t, k, guard = r.num_rows, 40, 2, 64
+    x, y, gy = (_rand(rows, d, dtype=dtype, seed=s) for rows, s in ((t, 2), (n, 3), (t, 4)))
+    rows = r.rows.clone()
+    rows[0, 0], rows[1, 1], rows[2, 0], rows[3, 1], rows[4, 0] = n, n + guard - 1, 2**31 - 1, -1, -5
+    inside = (rows >= 0) & (rows < n)
+    at = rows.long()
+    token = torch.arange(t, device="cuda").view(-1, 1).expand(t, k)
+    for counts, offsets in ((r.counts, r.offsets), (r.counts + 1000, r.offsets), (r.counts - 500, r.offsets),
+                            (r.counts, r.offsets - 9), (r.counts, r.offsets + n), (r.counts * 0 - 2**40, r.offsets * 2**40)):
+        def buffer():
+            b = torch.full((guard + n + guard, d), 7.0, dtype=dtype, device="cuda")
+            return b, b[guard:guard + n]
+
+        buf, out = buffer()
+        _lib.check(lib.rb_nvfp4_token_dispatch(x.data_ptr(), code, t, d, d, rows.data_ptr(), k, counts.data_ptr(),
+                                               offsets.data_ptr(), 4, out.data_ptr(), n, d, stream), "dispatch")
+        assert (buf[:guard] == 7).all() and (buf[-guard:] == 7).all()
+        if counts is r.counts and offsets is r.offsets:
+            assert torch.equal(out[at[inside]], x[token[inside]])
+        buf, out = buffer()
+        gw = torch.full((t, k), 7.0, device="cuda")
+        _lib.check(lib.rb_nvfp4_token_combine_backward(gy.data_ptr(), d, y.data_ptr(), d, code, t, d, rows.data_ptr(), k,
+                                                       r.weights.data_ptr(), counts.data_ptr(), offsets.data_ptr(), 4,
+                                                       out.data_ptr(), n, d, gw.data_ptr(), stream), "combine backward")
+        assert (buf[:guard] == 7).all() and (buf[-guard:] == 7).all()
+        assert (gw[~inside] == 0).all()
+        prod = gy.double().unsqueeze(1) * torch.where(inside.unsqueeze(-1), y.double()[at.clamp(0, n - 1)], 0.0)
+        assert ((gw.double() - prod.sum(-1)).abs() <= d * 2.0**-24 * prod.abs().sum(-1)).all()
+        if counts is r.counts and offsets is r.offsets:
+            want = (gy.float()[token[inside]] * r.weights[inside].unsqueeze(-1)).to(dtype)
+            assert torch.equal(out[at[inside]], want)
+        # The combine reads through the same rows.
+        buf = torch.full((guard + t + guard, d), 7.0, dtype=dtype, device="cuda")
+        out = buf[guard:guard + t]
+        _lib.check(lib.rb_nvfp4_token_combine(y.data_ptr(), code, n, d, d, rows.data_ptr(), k, r.weights.data_ptr(),
+                                              None, 0, out.data_ptr(), t, d, stream), "combine")
+        assert (buf[:guard] == 7).all() and (buf[-guard:] == 7).all()
+        terms = torch.where(inside.unsqueeze(-1), y.double()[at.clamp(0, n - 1)], 0.0) * r.weights.double().unsqueeze(-1)
+        hs = torch.finfo(dtype).eps / 2
+        assert ((out.double() - terms.sum(1)).abs()
+                <= hs * terms.sum(1).abs() * 1.01 + (k + 2) * 2.0**-24 * terms.abs().sum(1)).all()
