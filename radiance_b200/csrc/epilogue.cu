@@ -103,11 +103,11 @@ constexpr int kBwdLanes = 32;  // threads along a row, 8 columns each: a block c
 constexpr int kBwdRows = 8;    // rows a block reads at once
 constexpr int kBwdBlocksPerSm = 3;
 
-// Rows of a thread in flight: three of bf16, two of fp32 (a third would be spilled).
+// Rows of a thread in flight: three of bf16, two of fp32 (a few registers of fp32 are spilled as it is).
 template <typename T>
 constexpr int kBwdBatchOf = sizeof(T) == 2 ? 3 : 2;
 
-// 16384 x 5632 bf16 with the bias gradient: without an activation 64 us, relu^2 91, silu 90, GELU 101, against 57 and
+// 16384 x 5632 bf16 with the bias gradient: without an activation 63 us, relu^2 91, silu 91, GELU 104, against 57 and
 // 86 for the bytes at the copy's rate.  Four blocks to an SM with a row or two in flight: 69 to 77, 90 to 96, 97
 // to 100, 104 to 108; two blocks with four rows: 66, 89, 97, 108.
 template <typename T, int kAct, bool kVec>
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kBwdLanes* kBwdRows, kBwdBlocksPerSm) epilogue
           if constexpr (kAct != RB_ACT_NONE) zraw[u].get(zv);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            if constexpr (kAct != RB_ACT_NONE) g[j] = __fmul2_rn(g[j], act_derivative2<kAct>(zv[j]));
+            if constexpr (kAct != RB_ACT_NONE) g[j] = __fmul2_rn(g[j], act_derivative2<kAct, sizeof(T) == 4>(zv[j]));
             sum[j] = __fadd2_rn(sum[j], g[j]);
           }
           m = max(m, Io<T>::store8(dz + r * a.ldo + c, g));
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kBwdLanes* kBwdRows, kBwdBlocksPerSm) epilogue
           float v = Io<T>::load(dy + r * a.ldg + c + j);
           if (a.drop.seed != nullptr)
             v = dropout1(v, (uint64_t)(r * a.cols + c + j), key, a.drop.below, a.drop.scale);
-          if constexpr (kAct != RB_ACT_NONE) v *= act_derivative2<kAct>(both(Io<T>::load(z + r * a.ldz + c + j))).x;
+          if constexpr (kAct != RB_ACT_NONE) v *= act_derivative2<kAct, sizeof(T) == 4>(both(Io<T>::load(z + r * a.ldz + c + j))).x;
           if (j & 1) sum[j / 2].y += v;
           else sum[j / 2].x += v;
           m = max(m, Io<T>::store(dz + r * a.ldo + c + j, v));

@@ -970,10 +970,10 @@ __device__ __forceinline__ void box_add8(float2* v, uint32_t row_addr, int j, ui
   }
 }
 
-template <int kAct>
+template <int kAct, bool kExact>
 __device__ __forceinline__ void act32(float2 (&v)[16]) {
 #pragma unroll
-  for (int i = 0; i < 16; i += 8) act_batch<kAct, 8>(v + i);
+  for (int i = 0; i < 16; i += 8) act_batch<kAct, kExact, 8>(v + i);
 }
 
 // 32 accumulator columns of this lane's row (r), columns col0 .. col0 + 31 of the output, at the box's
@@ -1002,11 +1002,11 @@ __device__ __forceinline__ void fused_columns(const uint32_t* r, float alpha, co
     for (int j = 0; j < 4; ++j) box_store8<kF32>(v + 4 * j, zrow_addr, j0 + j, sw);
   }
   switch (g.act) {
-    case RB_ACT_RELU: act32<RB_ACT_RELU>(v); break;
-    case RB_ACT_RELU2: act32<RB_ACT_RELU2>(v); break;
-    case RB_ACT_SILU: act32<RB_ACT_SILU>(v); break;
-    case RB_ACT_GELU: act32<RB_ACT_GELU>(v); break;
-    case RB_ACT_GELU_TANH: act32<RB_ACT_GELU_TANH>(v); break;
+    case RB_ACT_RELU: act32<RB_ACT_RELU, kF32>(v); break;
+    case RB_ACT_RELU2: act32<RB_ACT_RELU2, kF32>(v); break;
+    case RB_ACT_SILU: act32<RB_ACT_SILU, kF32>(v); break;
+    case RB_ACT_GELU: act32<RB_ACT_GELU, kF32>(v); break;
+    case RB_ACT_GELU_TANH: act32<RB_ACT_GELU_TANH, kF32>(v); break;
     default: break;
   }
   if (g.drop.seed != nullptr) {

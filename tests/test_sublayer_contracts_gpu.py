@@ -389,3 +389,69 @@ def test_a_wrong_plan_writes_nothing_outside(nv, d, dtype):
         hs = torch.finfo(dtype).eps / 2
         assert ((out.double() - terms.sum(1)).abs()
                 <= hs * terms.sum(1).abs() * 1.01 + (k + 2) * 2.0**-24 * terms.abs().sum(1)).all()
+
+
+# ------------------------------------------------------------------------------------------------
+# Accuracy of the activations, relative to their own values
+# ------------------------------------------------------------------------------------------------
+
+REACH = {"silu": 80.0, "gelu": 12.0, "gelu_tanh": 9.0}  # beyond, results leave fp32's normal numbers on the left
+
+
+def _grid(act, n=8192):
+    """Even steps over the range, and magnitudes down to 2^-30 of either sign."""
+    line = torch.linspace(-REACH[act], REACH[act], n - 1024, device="cuda")
+    small = 2.0 ** torch.linspace(-30, 0, 512, device="cuda")
+    return torch.cat([line, small, -small])
+
+
+def _parts(z, act):
+    """The value, and the derivative's two terms, in float64."""
+    s = {"silu": lambda: torch.sigmoid(z), "gelu": lambda: 0.5 * torch.special.erfc(-z * 0.5**0.5),
+         "gelu_tanh": lambda: torch.sigmoid(2 * (2 / torch.pi) ** 0.5 * (z + 0.044715 * z**3))}[act]()
+    up = {"silu": lambda: s * torch.sigmoid(-z), "gelu": lambda: torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5,
+          "gelu_tanh": lambda: (s * torch.sigmoid(-2 * (2 / torch.pi) ** 0.5 * (z + 0.044715 * z**3))
+                                * 2 * (2 / torch.pi) ** 0.5 * (1 + 3 * 0.044715 * z * z))}[act]()
+    return z * s, s, z * up
+
+
+def _exact_room(act):
+    # In units of 2^-23 of the value: the exponential 2, the reciprocal 1 (times at most 2.6 where GELU's tail
+    # follows it), GELU's polynomial 1.1, and half of one for each of at most six roundings: under 9.
+    return 9 * 2.0**-23
+
+
+@pytest.mark.parametrize("act", list(REACH))
+def test_fp32_activations_are_accurate_everywhere(nv, act):
+    z = _grid(act)
+    a, b = nv.quantize(torch.zeros(128, 64, device="cuda"), -1), nv.quantize(torch.zeros(z.numel(), 64, device="cuda"), -1)
+    y, pre = nv.epilogue_mm(a, b, bias=z, activation=act, out_dtype=torch.float32, save_preact=True)  # 0 + bias
+    assert torch.equal(pre[0], z) and torch.equal(y, y[:1].expand_as(y))
+    value, s, t = _parts(z.double(), act)
+    assert ((y[0].double() - value).abs() <= _exact_room(act) * value.abs()).all()
+    d = nv.epilogue_backward(torch.ones(1, z.numel(), device="cuda"), z[None], activation=act)[0][0].double()
+    # Each term as the value; the sum is one rounding, the second term's factors two more.
+    assert ((d - s - t).abs() <= (_exact_room(act) + 1.5 * 2.0**-23) * (s + t.abs())).all()
+
+
+@pytest.mark.parametrize("act", list(REACH))
+def test_bf16_activations_are_rounded_about_once(nv, act):
+    """Before its one rounding GELU is off by 7.5e-8 of |z| near 0 and 3.8e-4 of itself far out on the left, the
+    others as in fp32 but for the exponent's roundings: 2^-23 of an exponent of at most 127."""
+    z = _grid(act).bfloat16()
+    a, b = nv.quantize(torch.zeros(128, 64, device="cuda"), -1), nv.quantize(torch.zeros(z.numel(), 64, device="cuda"), -1)
+    y = nv.epilogue_mm(a, b, bias=z, activation=act)[0].double()
+    zd = z.double()
+    value, s, t = _parts(zd, act)
+    room = 2.0**-20 + 127 * 2.0**-23
+    # GELU's tail q carries into z > 0 as z (1 - q) and into z < 0 as z q.
+    q = torch.minimum(s, 1 - s) if act == "gelu" else torch.zeros_like(s)
+    tail = torch.minimum(3.9e-4 * q, torch.full_like(q, 8e-8)) if act == "gelu" else q
+    err = room * value.abs() + tail * zd.abs()
+    assert ((y - value).abs() <= 2.0**-8 * (value.abs() + err) + err).all()
+    d = nv.epilogue_backward(torch.ones(1, z.numel(), dtype=torch.bfloat16, device="cuda"), z[None],
+                             activation=act)[0][0].double()
+    # 1 - s is taken from the rounded s here: 2^-23 of 1, times |z| times its factor (its slope).
+    slope = {"gelu": 0.0, "silu": 1.0, "gelu_tanh": 1.6 + 0.22 * zd * zd}[act]
+    err = room * (s + t.abs()) + tail + 2.0**-22 * s * zd.abs() * slope
+    assert ((d - s - t).abs() <= 2.0**-8 * ((s + t).abs() + err) + err).all()
