@@ -46,10 +46,15 @@ def _call(what: str, device: torch.device, fn, *args) -> None:
 
 
 def _tracked(*tensors: torch.Tensor | None) -> bool:
-    """Whether autograd follows one of these: in reverse (it requires a gradient) or forward mode (it has a tangent)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
-    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    """Whether autograd follows one of these: in reverse (it requires a gradient) or forward mode (it has a tangent,
+    which can be only inside a ``dual_level``: asking each tensor outside one would cost a third of a microsecond)."""
+    reverse, forward = torch.is_grad_enabled(), getattr(forward_ad, "_current_level", 0) >= 0
+    if reverse or forward:
+        for t in tensors:
+            if t is not None and ((reverse and t.requires_grad)
+                                  or (forward and forward_ad.unpack_dual(t).tangent is not None)):
+                return True
+    return False
 
 
 class _Refuse(torch.autograd.Function):
@@ -80,13 +85,8 @@ class _NoGradient(torch.autograd.Function):
         raise RuntimeError(f"{ctx.what} has no gradient formula: FP4Linear differentiates it")
 
 
-def _functional(what: str, call, out: torch.Tensor | None, kwargs, *tensors):
-    """``call(*tensors, out=out, **kwargs)``, refused or without a gradient where autograd follows a tensor."""
-    if not _tracked(out, *tensors):
-        result = call(*tensors, out=out, **kwargs)
-        if out is not None:  # written behind autograd's back: whoever saved it for backward must learn of it
-            torch.autograd.graph.increment_version(out)
-        return result
+def _no_gradient(what: str, call, out: torch.Tensor | None, kwargs, *tensors):
+    """``call(*tensors, out=None, **kwargs)`` for tensors that autograd follows; refused with an ``out``."""
     if out is not None:
         raise ValueError(f"{what}: out= cannot be differentiated, and one of its tensors requires a gradient")
     return _NoGradient.apply(what, call, dict(kwargs, out=None), *tensors)
@@ -282,12 +282,14 @@ def epilogue_mm(a: NVFP4Tensor, b: NVFP4Tensor, *, bias: torch.Tensor | None = N
     ``epilogue_backward`` takes.  No gradient formula (``FP4Linear`` has one): where ``bias`` or ``residual``
     requires a gradient, the result raises in backward, and ``out`` is refused.
     """
-    return _functional("nvfp4.epilogue_mm", _epilogue_mm, out,
-                       dict(a=a, b=b, activation=activation, dropout_p=dropout_p, seed=seed, out_dtype=out_dtype,
-                            save_preact=save_preact), bias, residual)
+    if _tracked(bias, residual, out):
+        return _no_gradient("nvfp4.epilogue_mm", _epilogue_mm, out,
+                            dict(a=a, b=b, activation=activation, dropout_p=dropout_p, seed=seed, out_dtype=out_dtype,
+                                 save_preact=save_preact), bias, residual)
+    return _epilogue_mm(bias, residual, a, b, activation, dropout_p, seed, out_dtype, out, save_preact)
 
 
-def _epilogue_mm(bias, residual, *, a, b, activation, dropout_p, seed, out_dtype, out, save_preact):
+def _epilogue_mm(bias, residual, a, b, activation, dropout_p, seed, out_dtype, out, save_preact):
     what = "nvfp4.epilogue_mm"
     ap, bp = a.packed, b.packed
     _require_cuda(ap, what)
@@ -315,7 +317,8 @@ def _epilogue_mm(bias, residual, *, a, b, activation, dropout_p, seed, out_dtype
     if residual is not None:
         _like("residual", residual, (m, n), out_dtype, dev, what)
     ldo = ldr = n
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(m, n, dtype=out_dtype, device=dev)
     else:
         _like("out", out, (m, n), out_dtype, dev, what)
@@ -335,6 +338,8 @@ def _epilogue_mm(bias, residual, *, a, b, activation, dropout_p, seed, out_dtype
           None if residual is None else residual.data_ptr(), ldr, None if z is None else z.data_ptr(), n,
           out.data_ptr(), out_code, ldo)
     _trace.end(tok)
+    if given:
+        torch.autograd.graph.increment_version(out)  # written behind autograd's back: who saved it must learn of it
     return (out, z) if save_preact else out
 
 
@@ -349,11 +354,14 @@ def epilogue_backward(grad_y: torch.Tensor, preact: torch.Tensor | None = None, 
     sums.  ``seed`` is the forward call's.  Returns ``(grad_z, global_scale_of(grad_z), sums or None)``.
     The gradient of the residual is ``grad_y`` itself.  No gradient formula, as ``epilogue_mm``.
     """
-    return _functional("nvfp4.epilogue_backward", _epilogue_backward, out,
-                       dict(activation=activation, dropout_p=dropout_p, seed=seed, bias_grad=bias_grad), grad_y, preact)
+    if _tracked(grad_y, preact, out):
+        return _no_gradient("nvfp4.epilogue_backward", _epilogue_backward, out,
+                            dict(activation=activation, dropout_p=dropout_p, seed=seed, bias_grad=bias_grad), grad_y,
+                            preact)
+    return _epilogue_backward(grad_y, preact, activation, dropout_p, seed, bias_grad, out)
 
 
-def _epilogue_backward(grad_y, preact, *, activation, dropout_p, seed, bias_grad, out):
+def _epilogue_backward(grad_y, preact, activation, dropout_p, seed, bias_grad, out):
     what = "nvfp4.epilogue_backward"
     _require_cuda(grad_y, what)
     code, act = _dtype_of(grad_y, what), _activation_code(activation, what)
@@ -373,7 +381,8 @@ def _epilogue_backward(grad_y, preact, *, activation, dropout_p, seed, bias_grad
             raise ValueError(f"{what}: dropout needs the forward call's seed")
         seed = _seed_tensor(seed, dev, what)
     ldo = cols
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(rows, cols, dtype=grad_y.dtype, device=dev)
     else:
         _like("out", out, (rows, cols), grad_y.dtype, dev, what)
@@ -393,4 +402,6 @@ def _epilogue_backward(grad_y, preact, *, activation, dropout_p, seed, bias_grad
           code, rows, cols, act, p, seed.data_ptr() if p > 0.0 else None, out.data_ptr(), ldo, gs.data_ptr(),
           None if sums is None else sums.data_ptr(), ws.data_ptr(), need)
     _trace.end(tok)
+    if given:
+        torch.autograd.graph.increment_version(out)
     return out, gs, sums
