@@ -143,13 +143,13 @@ __device__ __forceinline__ float2 logistic_power(float2 z) {
   const float2 f = __ffma2_rn(e, __fmul2_rn(lo, both(kLn2)), e);
   return make_float2(fabsf(x.x) < 126.0f ? f.x : e.x, fabsf(x.y) < 126.0f ? f.y : e.y);
 }
-// 1 - s for s = 1 / (1 + e).  kExact: e s, which does not cancel where s nears 1 (past 2^126 it is 1).
+// 1 - s for s = 1 / (1 + e).  kExact: e s where s is past 2/3 and 1 - s would cancel.
 template <bool kExact>
 __device__ __forceinline__ float2 one_minus(float2 s, float2 e) {
   const float2 d = __ffma2_rn(s, both(-1.0f), both(1.0f));
   if constexpr (!kExact) return d;
   const float2 f = __fmul2_rn(e, s);
-  return make_float2(e.x < 8.5e37f ? f.x : d.x, e.y < 8.5e37f ? f.y : d.y);
+  return make_float2(e.x < 0.5f ? f.x : d.x, e.y < 0.5f ? f.y : d.y);
 }
 
 // The normal distribution's tail q = Phi(-|z|) = erfc(|z| / sqrt 2) / 2 and e = exp(-z^2 / 2), as q = e t P(t),
